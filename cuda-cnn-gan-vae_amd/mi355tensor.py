@@ -23,6 +23,10 @@ class MtTensor(C.Structure):
     _fields_ = [("p", C.c_void_p), ("w", C.c_uint32), ("z", C.c_uint32), ("y", C.c_uint32), ("x", C.c_uint32)]
 
 
+class MtPackedTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("w", C.c_uint32), ("z", C.c_uint32), ("y", C.c_uint32), ("x", C.c_uint32)]
+
+
 class TensorError(RuntimeError):
     """A non-zero status of the C ABI (the C++ classes `throw` a message in the same place)."""
 
@@ -268,6 +272,54 @@ class CTensor:
             pass
 
 
+class CPackedTensor:
+    """Device-resident [W,Z,Y,X] activation kept in 8 bits (see mt_pack): 1.0625 bytes per element.  Filled by CTensorMath.Pack or
+    by a forward pass that is asked to keep its input, read by CTensorMath.Unpack and the backward passes that take it."""
+
+    def __init__(self, size_w=1, size_z=1, size_y=1, size_x=1):
+        self.shape = (int(size_w), int(size_z), int(size_y), int(size_x))
+        self.nbytes = self.bytes_of(self.shape)
+        self.ptr = C.c_void_p()
+        self.owned = True
+        call("mt_malloc", C.byref(self.ptr), C.c_size_t(self.nbytes))
+
+    @staticmethod
+    def bytes_of(shape):
+        n = C.c_uint64()
+        call("mt_packed_bytes", *(C.c_uint32(int(s)) for s in shape), C.byref(n))
+        return n.value
+
+    @classmethod
+    def wrap(cls, ptr, shape):
+        """Borrow bytes_of(shape) bytes of device memory, 16-byte aligned, that someone else owns."""
+        t = cls.__new__(cls)
+        t.shape, t.ptr, t.owned = tuple(int(s) for s in shape), C.c_void_p(ptr), False
+        t.nbytes = cls.bytes_of(t.shape)
+        return t
+
+    def ref(self):
+        r = self.__dict__.get("_ref")
+        if r is None:
+            if not self.ptr and self.nbytes:
+                raise RuntimeError("the tensor's device memory has been freed")
+            self._desc = MtPackedTensor(self.ptr.value, *self.shape)
+            r = self._ref = C.byref(self._desc)
+        return r
+
+    def free(self):
+        if self.owned and self.ptr:
+            call("mt_free", self.ptr)
+            self.ptr = C.c_void_p()
+            self.__dict__.pop("_ref", None)
+            self.__dict__.pop("_desc", None)
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 def _d(t):
     return t.ref()
 
@@ -436,6 +488,15 @@ class CTensorMath:
     def SetTimeStep(out, inp, time_step):
         call("mt_set_time_step", _d(out), _d(inp), _d(time_step))
 
+    # ---- activations in 8 bits (no counterpart in the reference)
+    @staticmethod
+    def Pack(out, inp):
+        call("mt_pack", _d(out), _d(inp))
+
+    @staticmethod
+    def Unpack(out, inp):
+        call("mt_unpack", _d(out), _d(inp))
+
     @staticmethod
     def CreateDropOutMatrix(out, drop_out, seed):
         call("mt_create_drop_out_matrix", _d(out), _f(drop_out), C.c_uint64(seed))
@@ -557,6 +618,29 @@ class Fused:
     def ConvolutionBackwardWeightsSum(dkernel, dkernel_x, dkernel_y, dkernel_z, dkernel_amount, dbias, image, delta, stride_x, stride_y, padding_x, padding_y):
         call("mt_convolution_backward_weights_sum", _d(dkernel), _i(dkernel_x), _i(dkernel_y), _i(dkernel_z), _u(dkernel_amount), _d(dbias), _d(image),
              _d(delta), _i(stride_x), _i(stride_y), _i(padding_x), _i(padding_y))
+
+    @staticmethod
+    def LayerNormForward(out, inp, gamma, beta, mean=None, ivar=None, packed=None, epsilon=1e-6, func=None):
+        """Rows as gamma names them ([1,Z,Y,X], [1,1,Y,X] or [1,1,1,X]) normalised by their own statistics.  mean, ivar: kept for
+        the backward pass; packed: a CPackedTensor that receives the input in 8 bits."""
+        opt = lambda t: _d(t) if t is not None else None
+        call("mt_layernorm_forward_func", _d(out), _d(inp), _d(gamma), _d(beta), opt(mean), opt(ivar), opt(packed), _f(epsilon), C.c_int(FUNC[func]))
+
+    @staticmethod
+    def LayerNormBackward(error, dgamma, dbeta, delta, gamma, inp, mean, ivar, beta=None, func=None, accumulate=True):
+        """inp: the forward pass's input, as a CTensor or as the CPackedTensor that it left.  accumulate: dgamma and dbeta are added
+        to (as the other backward calls do) or overwritten."""
+        opt = lambda t: _d(t) if t is not None else None
+        args = (_d(error), opt(dgamma), opt(dbeta), _d(delta), _d(gamma), opt(beta), _d(inp), _d(mean), _d(ivar), C.c_int(FUNC[func]), C.c_int(1 if accumulate else 0))
+        if isinstance(inp, CPackedTensor):
+            call("mt_layernorm_backward_packed_func", *args)
+        else:
+            call("mt_layernorm_backward_func", *args)
+
+    @staticmethod
+    def LinearBackwardWeightsSum(dweight, dbias, inp, delta, accumulate=True):
+        """Weight and bias gradient of a linear layer, summed over the batch, from its input kept in 8 bits (a CPackedTensor)."""
+        call("mt_linear_backward_weights_sum_packed", _d(dweight), _d(dbias) if dbias is not None else None, _d(inp), _d(delta), C.c_int(1 if accumulate else 0))
 
     @staticmethod
     def BatchNormForwardInfer(out, inp, gamma, beta, mean, variable, epsilon=1e-6, func=None):

@@ -51,6 +51,12 @@ typedef struct {
   uint32_t w, z, y, x;
 } mt_u32_tensor;
 
+/* An activation kept in 8 bits between the forward and the backward pass (mt_pack).  No counterpart in the reference. */
+typedef struct {
+  void *p; /* device pointer, 16-byte aligned, mt_packed_bytes(w,z,y,x) bytes */
+  uint32_t w, z, y, x;
+} mt_packed_tensor;
+
 enum {
   MT_OK = 0,
   MT_E_NO_KERNELS = 1,   /* kernel_amount == 0                                  (cpu/ctensorconv.h:88,199,321)  */
@@ -383,6 +389,57 @@ int mt_batchnorm_backward_func_keep(const mt_tensor *error, const mt_tensor *dga
 int mt_convolution_backward_weights_sum(const mt_tensor *dkernel, int32_t dkernel_x, int32_t dkernel_y, int32_t dkernel_z,
                                         uint32_t dkernel_amount, const mt_tensor *dbias, const mt_tensor *image,
                                         const mt_tensor *delta, int32_t stride_x, int32_t stride_y, int32_t padding_x, int32_t padding_y);
+
+/* ---- layer normalisation: rows of values normalised by their own mean and variance ----
+ * No counterpart in the reference: its batch normalisation (netlayer/cnetlayerbatchnormalization.cu.h:268-380) takes the
+ * statistics of an element over the batch, these entry points take the statistics of a row of one sample, so that a
+ * sample's result does not depend on the batch it is in.
+ * gamma names the row: [1,Z,Y,X] of the input's sizes (a row is a whole sample), [1,1,Y,X] (a plane; the features of a
+ * linear layer's output [B,1,Out,1]) or [1,1,1,X].  With N values per row:
+ *   mean = sum(x)/N, ivar = 1/sqrt(sum((x-mean)^2)/N + epsilon), xhat = (x-mean)*ivar, output = func(gamma*xhat + beta).
+ * mean and ivar hold one value per row: the input's sizes with 1 in place of those that the row spans.  Sums are fp32, taken in
+ * an order that depends on the sizes only: the same call gives the same bits.
+ * A NaN or an infinity in a row makes that row NaN (and the parameter gradients it adds to).  Rows of at most 2^31 - 17 values.
+ * No result may share memory with another tensor, but for the two cases named below.
+ *
+ * mt_layernorm_forward_func: mean and ivar (NULL to skip) are what the backward pass needs.  output may be the same tensor as
+ *   the input.  packed_input (NULL to skip) receives the input in 8 bits (as mt_pack would leave it), in the same pass
+ *   over it where the sizes allow. */
+int mt_layernorm_forward_func(const mt_tensor *output, const mt_tensor *input, const mt_tensor *gamma, const mt_tensor *beta, const mt_tensor *mean,
+                              const mt_tensor *ivar, const mt_packed_tensor *packed_input, float epsilon, int func);
+/* The backward pass (no counterpart in the reference).  delta: the gradient of func(gamma*xhat + beta); with
+ * g = delta*func'(gamma*xhat + beta) and u = g*gamma
+ *   error = ivar*(u - sum(u)/N - xhat*sum(u*xhat)/N) over each row, dgamma = sum over the rows of g*xhat, dbeta of g.
+ * accumulate: 1 adds the two sums to what dgamma and dbeta (sizes of gamma, NULL to skip) hold, as the other backward entry
+ * points do; 0 overwrites it.  input, mean, ivar: as the forward pass read and left them.  beta is needed unless func is
+ * MT_F_NONE / MT_F_LINEAR.  `error` may be the same tensor as `delta`. */
+int mt_layernorm_backward_func(const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
+                               const mt_tensor *beta, const mt_tensor *input, const mt_tensor *mean, const mt_tensor *ivar, int func, int accumulate);
+/* The same with the input as mt_pack (or the forward pass) keeps it in 8 bits: xhat is taken from the packed values, mean and
+ * ivar are those of the fp32 input.  No counterpart in the reference. */
+int mt_layernorm_backward_packed_func(const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
+                                      const mt_tensor *beta, const mt_packed_tensor *input, const mt_tensor *mean, const mt_tensor *ivar, int func,
+                                      int accumulate);
+
+/* ---- activations in 8 bits ----
+ * No counterpart in the reference.  A training step keeps every layer's input until the backward pass; kept in 8 bits it takes
+ * 1.0625 bytes per element instead of 4.  128 consecutive elements of a sample (its Z*Y*X values in memory order; the last
+ * group of a sample may be shorter) share a lowest value and a step:
+ *   low = min, step = (max - low) * (1/255), q = (x - low) / step rounded to a whole number (half to even), 0..255,
+ *   value = low + step*q, computed in fp32: |value - x| <= step/2 and the rounding of the sum.
+ * A group of equal values comes back exactly; one whose range is below 3e-36 as its lowest value.  A group whose range is not a
+ * finite number (it holds a NaN or an infinity, or values 3.4e38 apart) comes back as NaN in every element.
+ * Layout, for callers that store or move packed tensors: W rows of ceil(n/16)*16 bytes (n = Z*Y*X; q in element order, then
+ * zeros), followed by W rows of ceil(n/128) pairs (low, step) of floats. */
+int mt_packed_bytes(uint32_t w, uint32_t z, uint32_t y, uint32_t x, uint64_t *bytes);   /* no counterpart in the reference */
+int mt_pack(const mt_packed_tensor *output, const mt_tensor *input);                    /* no counterpart in the reference */
+int mt_unpack(const mt_tensor *output, const mt_packed_tensor *input);                  /* no counterpart in the reference */
+/* CNetLayerLinear::TrainingBackward, weight and bias part (netlayer/cnetlayerlinear.cu.h:415-447), from an input kept in 8 bits:
+ * dweight [1,1,Out,In] (+)= sum over the batch of delta (x) value(input), dbias [1,1,Out,1] (NULL to skip) (+)= sum of delta;
+ * input [B,...] of In values per sample, delta [B,...] of Out values.  accumulate: 1 adds to what the gradients hold, 0 overwrites.
+ * The products are those of the fp32 numbers delta and step with the whole numbers q, summed in fp32; a gradient's bits depend
+ * on the sizes only.  A delta that is not a finite number makes its row of dweight NaN. */
+int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_tensor *dbias, const mt_packed_tensor *input, const mt_tensor *delta, int accumulate);
 
 /* TrainingResetDeltaWeight of every layer of a network (netlayer/cnetlayerconvolution.cu.h:522-526 and the same
  * function of the other layers) as one launch: Fill(tensors[i], value) for i < count. */

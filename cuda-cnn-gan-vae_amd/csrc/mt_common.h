@@ -240,6 +240,15 @@ inline bool valid_func(int func, bool allow_none) {
   return func >= 0 && func < 16 && base >= MT_F_SIGMOID && base <= MT_F_TANGENCE;
 }
 
+// The hardware hands workgroup L of a 1-D grid to XCD (L % 8), each XCD with its own L2.  Renumbering gives
+// XCD x the contiguous logical range [x*total/8, (x+1)*total/8), so blocks that share operand tiles (neighbouring
+// logical indices) meet in one L2 instead of eight.
+__device__ __forceinline__ uint32_t xcd_swizzle(uint32_t L, uint32_t total) {
+  uint32_t per = total / 8;
+  if (L >= per * 8) return L;
+  return (L % 8) * per + L / 8;
+}
+
 // 64-lane wavefront sum
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

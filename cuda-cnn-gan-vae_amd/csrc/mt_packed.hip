@@ -1,4 +1,4 @@
-// Activations in 8 bits: mt_pack, mt_unpack and the linear layer's weight gradient from a packed input.
+// Activations in 8 bits: mt_pack and mt_unpack.
 #include "mt_packed.h"
 
 namespace {
@@ -51,25 +51,6 @@ __global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackedView 
   }
 }
 
-// dweight[o][i] (+)= sum_b delta[b][o] * value[b][i], dbias[o] (+)= sum_b delta[b][o]: one thread per weight
-__global__ __launch_bounds__(THREADS) void linear_weights_kernel(float *dweight, float *dbias, const float *delta, PackedView in, uint32_t Out, bool accumulate) {
-  const uint32_t i = blockIdx.x * 64u + threadIdx.x % 64u;
-  for (uint32_t o = blockIdx.y * 4u + threadIdx.x / 64u; o < Out; o += gridDim.y * 4u) {
-    float acc = 0.f, sum = 0.f;
-    if (i < in.n || i == 0)
-      for (uint32_t b = 0; b < in.w; b++) {
-        const float d = delta[(size_t)b * Out + o];
-        if (i < in.n) acc += d * mt::unpack_value(in.pair[(size_t)b * in.groups + i / mt::PACK_GROUP], in.q[(size_t)b * in.pitch + i]);
-        sum += d;
-      }
-    if (i < in.n) {
-      const size_t e = (size_t)o * in.n + i;
-      dweight[e] = accumulate ? dweight[e] + acc : acc;
-    }
-    if (i == 0 && dbias) dbias[o] = accumulate ? dbias[o] + sum : sum;
-  }
-}
-
 }  // namespace
 
 extern "C" {
@@ -110,36 +91,6 @@ int mt_unpack(const mt_tensor *out, const mt_packed_tensor *in) {
   const size_t total = (size_t)v.w * v.n;
   unpack_kernel<<<blocks_for(total, THREADS), THREADS, 0, mt::stream()>>>(out->p, v, total);
   MT_LAUNCH_CHECK("mt_unpack");
-  return MT_OK;
-}
-
-int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_tensor *dbias, const mt_packed_tensor *input, const mt_tensor *delta, int accumulate) {
-  const char *name = "mt_linear_backward_weights_sum_packed";
-  if (mt::bad(dweight) || (dbias && mt::bad(dbias)) || mt::bad(input) || mt::bad(delta))
-    return mt::fail(MT_E_ARGUMENT, "%s: null tensor, or packed memory that is not 16-byte aligned", name);
-  PackedView v;
-  if (!mt::packed_view(input, &v)) return mt::fail(MT_E_UNAVAILABLE, "%s: a sample of 2^31 elements or more is not supported", name);
-  const uint64_t out = (uint64_t)delta->z * delta->y * delta->x;  // the layer's output may be seen under any sizes of Out values
-  if (dweight->w != 1 || dweight->z != 1 || dweight->x != v.n || dweight->y != out || delta->w != v.w)
-    return mt::fail(MT_E_SHAPE, "%s: dweight must be [1,1,Out,In], the input [B,...] of In values, delta [B,...] of Out values", name);
-  if (dbias && (dbias->w != 1 || dbias->z != 1 || dbias->x != 1 || dbias->y != out)) return mt::fail(MT_E_SHAPE, "%s: dbias must be [1,1,Out,1]", name);
-  const uint32_t Out = (uint32_t)out;
-  if (Out == 0) return MT_OK;
-  for (auto t : {dweight, dbias})
-    if (t && (mt::overlap(t, delta) || mt::overlap(t, v))) return mt::fail(MT_E_ARGUMENT, "%s: a gradient shares memory with an input", name);
-  if (dbias && mt::overlap(dbias, dweight)) return mt::fail(MT_E_ARGUMENT, "%s: dbias shares memory with dweight", name);
-  if (v.w == 0) {  // an empty batch: the sums are zero
-    if (accumulate) return MT_OK;
-    int rc = mt_fill(dweight, 0.f);
-    return rc || !dbias ? rc : mt_fill(dbias, 0.f);
-  }
-  mt::note_write(dweight);
-  mt::note_write(dbias);
-  mt::ProfileScope prof(name);
-  const unsigned gy = cdiv(Out, 4);
-  linear_weights_kernel<<<dim3(cdiv(v.n ? v.n : 1, 64), gy < 4096 ? gy : 4096), THREADS, 0, mt::stream()>>>(dweight->p, dbias ? dbias->p : nullptr, delta->p, v, Out,
-                                                                                                           accumulate != 0);
-  MT_LAUNCH_CHECK(name);
   return MT_OK;
 }
 

@@ -1,0 +1,314 @@
+// The linear layer's weight gradient from an input kept in 8 bits, on the bf16 matrix cores with fp32 results.
+//
+//   dweight[o][i] = sum_b delta[b][o] * (low[b][g] + step[b][g] * q[b][i]),  g = the group of 128 columns that i is in
+//                 = sum_b (delta * step)[b][o] * (q[b][i] - 128)  +  sum_b delta[b][o] * (low + 128 * step)[b][g]
+//
+// q - 128 is a whole number of 8 bits: exact in bf16.  delta * step, one fp32 product, is the exact sum of three bf16 numbers:
+// its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder exact).  Three bf16
+// matrix instructions therefore multiply what one fp32 product would, into fp32 accumulators, at a third of the bf16
+// rate (some 800 TFLOP/s) where the fp32 matrix instructions reach 157.  The second sum is one fp32 multiply-add per element of
+// delta on the way.
+//
+// A column tile is one group, so that a sample has one (low, step) in it.  A block is four wavefronts, each with its own 32 or
+// 64 rows (output features) and all 128 columns: no other wavefront needs its rows, so delta goes from memory to registers in
+// the lane layout of the matrix instruction and is scaled and cut there, never through LDS.  The columns, which all four
+// need, are turned into bf16 once and shared through LDS, eight samples of one column per 16 bytes: that is what a lane
+// reads.  The block takes 64 samples per step; the next step's columns are loaded before and written after the step's
+// products, the next 16 samples of delta are loaded before the products of the 16 in hand.
+#include "mt_packed.h"
+
+namespace {
+
+using mt::cdiv;
+using mt::PackedView;
+using mt::xcd_swizzle;
+
+constexpr int THREADS = 256;
+constexpr uint32_t KSTEP = 64;  // samples per step
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+// the next rows of an operand, at most `most` of the `left` that there are (none: left <= 0): what lies behind them reads as
+// zero.  most * row_bytes <= 2^31: 16 rows of delta, 64 of the packed bytes, fewer than 2^25 features.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void *p, int left, int most, uint32_t row_bytes) {
+  const uint32_t rows = __builtin_amdgcn_readfirstlane(max(0, min(left, most)));  // (a clamp is a vector instruction: back to a scalar)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)(rows * row_bytes), 0x00020000);
+}
+
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {  // the bf16 numbers of a (low half) and b, cut off
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+
+struct WgradArgs {
+  const float *delta;
+  PackedView in;
+  float *dweight, *dbias;    // split == 1: the gradients; else [split][Out*In] and [split][Out] partial sums
+  uint32_t Out, tiles_m, split, per_split;  // per_split: samples of one part, a multiple of KSTEP
+  bool accumulate;
+};
+
+template <int TM>
+struct WgradSums {
+  floatx16 acc[TM][4];           // matrix-core sums: 32 rows x 32 columns each
+  float offset[TM], bias[TM];    // the second sum and the sum of delta: row lane % 32, half of the samples each
+};
+
+// the product over the samples k0 ... k1; BIAS: the sum of delta too (the blocks of the first group)
+template <int TM, bool BIAS>
+__device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g, uint32_t m0, uint32_t k0, uint32_t k1, uintx4 (*cols)[KSTEP / 8][128], float2 (*scale)[KSTEP],
+                                                  WgradSums<TM> &sums) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 31u, half = lane >> 5;
+  const uint32_t steps = (k1 - k0 + KSTEP - 1) / KSTEP;
+  float d[8][TM];  // this lane's rows r * TM ... of eight samples
+  uint32_t voff[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) voff[j] = ((half * 8u + j) * a.Out + m0 + r * TM) * 4u;
+
+  auto load_delta = [&](uint32_t k) {
+    const auto rsrc = rows_rsrc(a.delta + (size_t)k * a.Out, (int)k1 - (int)k, 16, a.Out * 4u);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (TM == 2) {
+        const uintx2 v = __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)voff[j], 0, 0);
+        d[j][0] = __uint_as_float(v[0]);
+        d[j][TM - 1] = __uint_as_float(v[1]);
+      } else {
+        d[j][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)voff[j], 0, 0));
+      }
+    }
+  };
+  const uint32_t kg = tid / 32u, c4 = (tid & 31u) * 4u;  // this thread's eight samples and four columns of a step
+  uint32_t q[8];
+  uintx2 pair;
+  auto load_cols = [&](uint32_t k) {
+    const auto rsrc = rows_rsrc(a.in.q + (size_t)k * a.in.pitch, (int)k1 - (int)k, KSTEP, a.in.pitch);
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)((kg * 8u + j) * a.in.pitch + g * 128u + c4), 0, 0);
+    // (samples behind the end have a step and a lowest value of zero, whatever follows in memory)
+    pair = __builtin_amdgcn_raw_buffer_load_b64(rows_rsrc(a.in.pair + (size_t)k * a.in.groups, (int)k1 - (int)k, KSTEP, a.in.groups * 8u),
+                                                (int)((tid % KSTEP) * a.in.groups * 8u + g * 8u), 0, 0);
+  };
+  auto store_cols = [&](uint32_t buf) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = (float)((q[j] >> (8 * c)) & 255u) - 128.f;
+      uintx4 w;
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = upper_halves(v[2 * j], v[2 * j + 1]);
+      cols[buf][kg][c4 + c] = w;
+    }
+    if (tid < KSTEP) scale[buf][tid] = make_float2(__uint_as_float(pair.y), __builtin_fmaf(128.f, __uint_as_float(pair.y), __uint_as_float(pair.x)));
+  };
+
+  load_cols(k0);
+  load_delta(k0);
+  store_cols(0);
+  __syncthreads();
+  for (uint32_t s = 0; s < steps; s++) {
+    const uint32_t buf = s & 1u, k = k0 + s * KSTEP;
+    load_cols(k + KSTEP);
+#pragma unroll
+    for (int kk = 0; kk < 4; kk++) {
+      bf16x8 col[4];
+#pragma unroll
+      for (int n = 0; n < 4; n++) col[n] = __builtin_bit_cast(bf16x8, cols[buf][kk * 2 + half][n * 32 + r]);
+#pragma unroll
+      for (int m = 0; m < TM; m++) {
+        uintx4 cuts[3];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float x[2], y[2], z[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float v = d[2 * j + e][m];
+            const float2 sc = scale[buf][kk * 16 + half * 8u + 2 * j + e];
+            if (BIAS) sums.bias[m] += v;
+            sums.offset[m] = __builtin_fmaf(v, sc.y, sums.offset[m]);
+            x[e] = v * sc.x;
+            y[e] = x[e] - cut(x[e]);
+            z[e] = y[e] - cut(y[e]);
+          }
+          cuts[0][j] = upper_halves(x[0], x[1]);
+          cuts[1][j] = upper_halves(y[0], y[1]);
+          cuts[2][j] = upper_halves(z[0], z[1]);
+        }
+        // (the compiler would leave these sums for the end of the step and keep four times the registers of delta for them)
+        asm volatile("" : "+v"(sums.offset[m]));
+        if (BIAS) asm volatile("" : "+v"(sums.bias[m]));
+        if (m == TM - 1) load_delta(k + 16u * (kk + 1));
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+#pragma unroll
+          for (int n = 0; n < 4; n++)
+            sums.acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, cuts[p]), col[n], sums.acc[m][n], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // nothing of the next 16 samples moves up: the registers are full
+    }
+    store_cols(buf ^ 1u);
+    __syncthreads();
+  }
+}
+
+template <int TM>
+__global__ __launch_bounds__(THREADS, 2) void packed_wgrad_kernel(WgradArgs a) {
+  __shared__ uintx4 cols[2][KSTEP / 8][128];  // [eight samples][column]
+  __shared__ float2 scale[2][KSTEP];          // (step, low + 128 * step)
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, r = lane & 31u, half = lane >> 5;
+  // neighbouring blocks of an XCD share their rows of delta (the larger operand) and walk over the groups
+  uint32_t t = __builtin_amdgcn_readfirstlane(xcd_swizzle(blockIdx.x, gridDim.x));
+  const uint32_t g = t % a.in.groups;
+  t /= a.in.groups;
+  const uint32_t m0 = (t % a.tiles_m) * (128u * TM) + wave * (32u * TM), part = t / a.tiles_m;
+  const uint32_t k0 = part * a.per_split, k1 = min(a.in.w, k0 + a.per_split);
+  const bool bias = a.dbias != nullptr && g == 0;
+  WgradSums<TM> sums;
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    sums.offset[m] = sums.bias[m] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
+  }
+  if (bias)
+    packed_wgrad_loop<TM, true>(a, g, m0, k0, k1, cols, scale, sums);
+  else
+    packed_wgrad_loop<TM, false>(a, g, m0, k0, k1, cols, scale, sums);
+
+  float *dw = a.dweight, *db = a.dbias;
+  if (a.split > 1) {
+    dw += (size_t)part * a.Out * a.in.n;
+    if (db) db += (size_t)part * a.Out;
+  }
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    sums.offset[m] += __shfl_xor(sums.offset[m], 32, 64);
+    sums.bias[m] += __shfl_xor(sums.bias[m], 32, 64);
+    if (bias && half == 0 && m0 + r * TM + m < a.Out) {
+      float *p = db + m0 + r * TM + m;
+      *p = a.accumulate ? *p + sums.bias[m] : sums.bias[m];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const uint32_t row = 8u * (i / 4) + 4u * half + i % 4, o = m0 + row * TM + m;
+      const float c = __shfl(sums.offset[m], (int)row, 64);
+      if (o < a.Out)
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const uint32_t col = g * 128u + n * 32u + r;
+          if (col < a.in.n) {
+            float *p = dw + (size_t)o * a.in.n + col;
+            const float v = sums.acc[m][n][i] + c;
+            *p = a.accumulate ? *p + v : v;
+          }
+        }
+    }
+  }
+}
+
+// the parts of a split sum, added in their order: first the weights' n values, then the bias's Out
+__global__ __launch_bounds__(THREADS) void packed_wgrad_join_kernel(float *dweight, float *dbias, const float *partial, const float *partial_bias, uint32_t split, size_t n,
+                                                                   uint32_t Out, bool accumulate) {
+  const size_t i = (size_t)blockIdx.x * THREADS + threadIdx.x;
+  const bool weight = i < n;
+  if (!weight && (dbias == nullptr || i - n >= Out)) return;
+  const float *p = weight ? partial + i : partial_bias + (i - n);
+  float *out = weight ? dweight + i : dbias + (i - n);
+  const size_t stride = weight ? n : Out;
+  float s = 0.f;
+#pragma unroll 4
+  for (uint32_t k = 0; k < split; k++, p += stride) s += *p;
+  *out = accumulate ? *out + s : s;
+}
+
+// dbias alone, for a layer without input features
+__global__ __launch_bounds__(THREADS) void bias_only_kernel(float *dbias, const float *delta, uint32_t w, uint32_t Out, bool accumulate) {
+  const uint32_t o = blockIdx.x * THREADS + threadIdx.x;
+  if (o >= Out) return;
+  float s = 0.f;
+  for (uint32_t b = 0; b < w; b++) s += delta[(size_t)b * Out + o];
+  dbias[o] = accumulate ? dbias[o] + s : s;
+}
+
+mt::Workspace g_wgrad_ws;
+
+}  // namespace
+
+extern "C" {
+
+int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_tensor *dbias, const mt_packed_tensor *input, const mt_tensor *delta, int accumulate) {
+  const char *name = "mt_linear_backward_weights_sum_packed";
+  if (mt::bad(dweight) || (dbias && mt::bad(dbias)) || mt::bad(input) || mt::bad(delta))
+    return mt::fail(MT_E_ARGUMENT, "%s: null tensor, or packed memory that is not 16-byte aligned", name);
+  PackedView v;
+  if (!mt::packed_view(input, &v)) return mt::fail(MT_E_UNAVAILABLE, "%s: a sample of 2^31 elements or more is not supported", name);
+  const uint64_t out = (uint64_t)delta->z * delta->y * delta->x;  // the layer's output may be seen under any sizes of Out values
+  if (dweight->w != 1 || dweight->z != 1 || dweight->x != v.n || dweight->y != out || delta->w != v.w)
+    return mt::fail(MT_E_SHAPE, "%s: dweight must be [1,1,Out,In], the input [B,...] of In values, delta [B,...] of Out values", name);
+  if (dbias && (dbias->w != 1 || dbias->z != 1 || dbias->x != 1 || dbias->y != out)) return mt::fail(MT_E_SHAPE, "%s: dbias must be [1,1,Out,1]", name);
+  // a step's 64 samples are addressed with 32-bit offsets
+  if (v.n >= (1u << 25) || out >= (1u << 25)) return mt::fail(MT_E_UNAVAILABLE, "%s: 2^25 features or more are not supported", name);
+  const uint32_t Out = (uint32_t)out;
+  if (Out == 0) return MT_OK;
+  for (auto t : {dweight, dbias})
+    if (t && (mt::overlap(t, delta) || mt::overlap(t, v))) return mt::fail(MT_E_ARGUMENT, "%s: a gradient shares memory with an input", name);
+  if (dbias && mt::overlap(dbias, dweight)) return mt::fail(MT_E_ARGUMENT, "%s: dbias shares memory with dweight", name);
+  if (v.w == 0) {  // an empty batch: the sums are zero
+    if (accumulate) return MT_OK;
+    int rc = mt_fill(dweight, 0.f);
+    return rc || !dbias ? rc : mt_fill(dbias, 0.f);
+  }
+  mt::note_write(dweight);
+  mt::note_write(dbias);
+  mt::ProfileScope prof(name);
+  if (v.n == 0) {
+    if (dbias) bias_only_kernel<<<cdiv(Out, THREADS), THREADS, 0, mt::stream()>>>(dbias->p, delta->p, v.w, Out, accumulate != 0);
+    MT_LAUNCH_CHECK(name);
+    return MT_OK;
+  }
+  WgradArgs a{};
+  a.delta = delta->p; a.in = v; a.Out = Out; a.accumulate = accumulate != 0;
+  const bool wide = Out % 2 == 0 && Out > 128 && (size_t)cdiv(Out, 256) * v.groups * cdiv(v.w, 1024) >= 256;
+  a.tiles_m = cdiv(Out, wide ? 256 : 128);
+  const size_t tiles = (size_t)a.tiles_m * v.groups;
+  // few tiles: parts of the batch, at least 256 samples each, until the chip has its two blocks per compute unit
+  uint32_t split = 1;
+  if (tiles < 512) {
+    split = (uint32_t)(512 / tiles);
+    const uint32_t most = v.w / 256;
+    if (split > most) split = most;
+    if (split < 1) split = 1;
+  }
+  a.per_split = cdiv(cdiv(v.w, split), KSTEP) * KSTEP;
+  a.split = cdiv(v.w, a.per_split);
+  const size_t n = (size_t)Out * v.n;
+  float *ws = nullptr;
+  if (a.split > 1) {
+    int rc = mt::workspace_get(g_wgrad_ws, "packed weight gradient", a.split * (n + Out), &ws);
+    if (rc) return rc;
+    a.dweight = ws;
+    a.dbias = dbias ? ws + a.split * n : nullptr;
+    a.accumulate = false;
+  } else {
+    a.dweight = dweight->p;
+    a.dbias = dbias ? dbias->p : nullptr;
+  }
+  const size_t grid = tiles * a.split;
+  if (grid > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);
+  if (wide)
+    packed_wgrad_kernel<2><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  else
+    packed_wgrad_kernel<1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  MT_LAUNCH_CHECK(name);
+  if (a.split > 1) {
+    packed_wgrad_join_kernel<<<cdiv(n + Out, THREADS), THREADS, 0, mt::stream()>>>(dweight->p, dbias ? dbias->p : nullptr, ws, ws + a.split * n, a.split, n, Out, accumulate != 0);
+    MT_LAUNCH_CHECK(name);
+  }
+  return MT_OK;
+}
+
+}  // extern "C"

@@ -3,6 +3,13 @@
 //   mean = sum(x) / N,  ivar = 1 / sqrt(sum((x - mean)^2) / N + epsilon),  xhat = (x - mean) * ivar,  y = f(gamma * xhat + beta)
 // Backward, with g = delta * f'(gamma * xhat + beta) and u = g * gamma:
 //   error = ivar * (u - sum(u) / N - xhat * sum(u * xhat) / N),  dgamma = sum over the rows of g * xhat,  dbeta = of g
+//
+// All of it is bound by memory: the forward pass has to read x and write y, the backward pass to read delta and x and write the
+// error.  A row is therefore held in registers between its sums and its results wherever it fits (one to 1024 threads per row, up
+// to 32 values per thread); longer rows are cut into pieces that several blocks share, and their second look at x finds it in
+// the caches.  Variances are sums of squared deviations from the mean (two passes over registers), never E[x^2] - E[x]^2.
+#include <type_traits>
+
 #include "mt_packed.h"
 
 namespace {
@@ -12,110 +19,556 @@ using mt::PackedView;
 
 constexpr int THREADS = 256;
 
+// ---- sums over the lanes of a row (8, 16 or 64 lanes of a wavefront, or whole blocks); every lane gets the same bits ----------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+struct Sum {
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct Lowest {
+  static __device__ __forceinline__ float of(float a, float b) { return mt::min_nan(a, b); }
+};
+struct Highest {
+  static __device__ __forceinline__ float of(float a, float b) { return mt::max_nan(a, b); }
+};
+template <class Op, int L>
+__device__ __forceinline__ float over_lanes(float v) {
+  v = Op::of(v, dpp<0xb1>(v));                  // neighbours
+  v = Op::of(v, dpp<0x4e>(v));                  // pairs of a quad
+  v = Op::of(v, dpp<0x141>(v));                 // quads of eight lanes
+  if (L > 8) v = Op::of(v, dpp<0x140>(v));      // halves of sixteen
+  if (L > 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  if (L > 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  return v;
+}
+// over the L threads of a row; `part` (L / 64 values, rows of whole blocks) is used once: no second barrier
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float *part) {
+  v = over_lanes<Sum, L < 64 ? L : 64>(v);
+  if (L > 64) {
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int k = 1; k < L / 64; k++) v += part[k];
+  }
+  return v;
+}
+
+// ---- how the L threads of a row share its N values: E each, in vectors of four 4 * L apart, or singly L apart ----------------
+template <int L, int E, bool VEC>
+struct Share {
+  static constexpr int STEPS = VEC ? E / 4 : E, WIDTH = VEC ? 4 : 1;
+  static __device__ __forceinline__ uint32_t first(int j) { return (j * L + threadIdx.x % L) * WIDTH; }
+  // values behind the end read the last ones again and count as `other`
+  static __device__ __forceinline__ void load(float (&v)[E], const float *p, uint32_t N, float other) {
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+      const uint32_t i = first(j), at = min(i, N - WIDTH);
+      if (VEC) {
+        const float4 t = *reinterpret_cast<const float4 *>(p + at);
+        v[j * WIDTH] = t.x; v[j * WIDTH + WIDTH / 4] = t.y; v[j * WIDTH + WIDTH / 2] = t.z; v[j * WIDTH + WIDTH - 1] = t.w;
+      } else {
+        v[j] = p[at];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+#pragma unroll
+      for (int e = 0; e < WIDTH; e++) v[j * WIDTH + e] = first(j) < N ? v[j * WIDTH + e] : other;
+  }
+  static __device__ __forceinline__ void store(float *p, int j, const float *t) {
+    if (VEC)
+      *reinterpret_cast<float4 *>(p + first(j)) = make_float4(t[0], t[WIDTH / 4], t[WIDTH / 2], t[WIDTH - 1]);
+    else
+      p[first(j)] = t[0];
+  }
+};
+template <bool VEC>
+__device__ __forceinline__ void load_step(float *t, const float *p, uint32_t at) {
+  if (VEC) {
+    const float4 q = *reinterpret_cast<const float4 *>(p + at);
+    t[0] = q.x; t[1] = q.y; t[2] = q.z; t[3] = q.w;
+  } else {
+    t[0] = p[at];
+  }
+}
+
 // ---- where a row's input comes from in the backward pass: the fp32 tensor, or the 8 bits the forward pass kept ------------
 struct RowsF32 {
   const float *p;
   uint32_t N;
-  __device__ __forceinline__ float at(size_t row, uint32_t i) const { return p[row * N + i]; }
+  struct Row {
+    const float *p;
+    template <bool VEC>
+    __device__ __forceinline__ void step(float *t, uint32_t at) const { load_step<VEC>(t, p, at); }
+  };
+  __device__ __forceinline__ Row row(uint32_t r) const { return Row{p + (size_t)r * N}; }
 };
 struct RowsPacked {
   PackedView v;
   uint32_t N, per_sample;  // rows of one sample
-  __device__ __forceinline__ float at(size_t row, uint32_t i) const {
-    const size_t w = row / per_sample;
-    const uint32_t e = (uint32_t)(row - w * per_sample) * N + i;
-    return mt::unpack_value(v.pair[w * v.groups + e / mt::PACK_GROUP], v.q[w * v.pitch + e]);
+  struct Row {
+    const uint8_t *q;
+    const float2 *pair;
+    uint32_t first;  // the row's first value within its sample
+    template <bool VEC>
+    __device__ __forceinline__ void step(float *t, uint32_t at) const {
+      const uint32_t e = first + at;
+      const float2 s = pair[e / mt::PACK_GROUP];
+      if (VEC) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(q + e);
+#pragma unroll
+        for (int k = 0; k < 4; k++) t[k] = mt::unpack_value(s, (w >> (8 * k)) & 255u);
+      } else {
+        t[0] = mt::unpack_value(s, q[e]);
+      }
+    }
+  };
+  __device__ __forceinline__ Row row(uint32_t r) const {
+    const uint32_t w = per_sample == 1 ? r : r / per_sample;
+    return Row{v.q + (size_t)w * v.pitch, v.pair + (size_t)w * v.groups, (r - w * per_sample) * N};
   }
 };
 
-__device__ __forceinline__ float block_sum(float v, float *part) {
-  v = mt::wave_sum(v);
-  __syncthreads();  // part may still be read from the sum before
-  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
-  __syncthreads();
-  float s = 0.f;
-  for (uint32_t k = 0; k < blockDim.x / 64; k++) s += part[k];
-  return s;
+// the 8 bits of one vector per lane, 32 lanes a group: lanes behind the end of the row give
+// `valid` false; those behind the end of the sample write its padding
+__device__ __forceinline__ void pack_step(const PackedView &out, size_t sample, uint32_t e, bool valid, const float *t) {
+  float low = mt::min_nan(mt::min_nan(t[0], t[1]), mt::min_nan(t[2], t[3])), high = mt::max_nan(mt::max_nan(t[0], t[1]), mt::max_nan(t[2], t[3]));
+  low = over_lanes<Lowest, 32>(valid ? low : __int_as_float(0x7f800000));
+  high = over_lanes<Highest, 32>(valid ? high : __int_as_float(0xff800000));
+  const mt::PackScale s = mt::pack_scale(low, high);
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) w |= mt::pack_value(s, t[k]) << (8 * k);
+  if (valid || (e >= out.n && e < out.pitch)) *reinterpret_cast<uint32_t *>(out.q + sample * out.pitch + e) = valid ? w : 0u;
+  if (valid && e % mt::PACK_GROUP == 0) out.pair[sample * out.groups + e / mt::PACK_GROUP] = make_float2(s.low, s.step);
 }
 
-__global__ __launch_bounds__(THREADS) void ln_forward_kernel(float *out, const float *in, const float *gamma, const float *beta, float *mean_out, float *ivar_out,
-                                                             size_t rows, uint32_t N, float eps, int func) {
-  __shared__ float part[THREADS / 64];
-  for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float *x = in + row * N;
-    float s = 0.f;
-    for (uint32_t i = threadIdx.x; i < N; i += THREADS) s += x[i];
-    const float mean = block_sum(s, part) / (float)N;
-    s = 0.f;
-    for (uint32_t i = threadIdx.x; i < N; i += THREADS) {
-      const float d = x[i] - mean;
-      s += d * d;
-    }
-    const float ivar = 1.f / sqrtf(block_sum(s, part) / (float)N + eps);
-    for (uint32_t i = threadIdx.x; i < N; i += THREADS) out[row * N + i] = mt::apply_func_epilogue(func, gamma[i] * ((x[i] - mean) * ivar) + beta[i]);
-    if (threadIdx.x == 0) {
-      if (mean_out) mean_out[row] = mean;
-      if (ivar_out) ivar_out[row] = ivar;
-    }
+// ---- forward -------------------------------------------------------------------------------------------------------
+struct Forward {
+  float *out;
+  const float *in, *gamma, *beta;
+  float *mean, *ivar;  // null: not wanted
+  PackedView packed;
+  uint32_t rows, N, per_sample;
+  float eps;
+  int func;
+};
+
+// gamma * xhat + beta and the function, from x in registers
+template <int L, int E, bool VEC>
+__device__ __forceinline__ void normalise(const Forward &a, float *out, const float (&x)[E], float mean, float ivar, const float *gamma, const float *beta, uint32_t N) {
+  using S = Share<L, E, VEC>;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) {
+    if (S::first(j) >= N) continue;
+    float g[S::WIDTH], b[S::WIDTH], y[S::WIDTH];
+    load_step<VEC>(g, gamma, S::first(j));
+    load_step<VEC>(b, beta, S::first(j));
+#pragma unroll
+    for (int e = 0; e < S::WIDTH; e++) y[e] = g[e] * ((x[j * S::WIDTH + e] - mean) * ivar) + b[e];
+    mt::apply_func_epilogue_many<S::WIDTH>(a.func, y);
+    S::store(out, j, y);
   }
 }
 
-// the gradient in front of the function
-__device__ __forceinline__ float front(int func, float delta, float gamma, float xhat, const float *beta, uint32_t i) {
-  return func == MT_F_NONE ? delta : delta * mt::apply_func(MT_F_DIFFERENTIAL + func, gamma * xhat + beta[i]);
+// rows that fit the registers of L threads
+template <int L, int E, bool VEC, bool PACK>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a) {
+  using S = Share<L, E, VEC>;
+  constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
+  __shared__ float part[2][L / 64 + 1];
+  const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
+  const bool mine = want < a.rows;
+  float x[E];
+  S::load(x, a.in + (size_t)row * a.N, a.N, 0.f);
+  if (PACK) {
+    const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N;
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++)
+      if (mine) pack_step(a.packed, w, e0 + S::first(j), S::first(j) < a.N, x + j * S::WIDTH);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < E; k++) s += x[k];
+  const float mean = row_sum<L>(s, part[0]) / (float)a.N;
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++)
+#pragma unroll
+    for (int e = 0; e < S::WIDTH; e++) {
+      const float d = S::first(j) < a.N ? x[j * S::WIDTH + e] - mean : 0.f;
+      s += d * d;
+    }
+  const float ivar = 1.f / sqrtf(row_sum<L>(s, part[1]) / (float)a.N + a.eps);
+  if (!mine) return;
+  normalise<L, E, VEC>(a, a.out + (size_t)row * a.N, x, mean, ivar, a.gamma, a.beta, a.N);
+  if (threadIdx.x % L == 0) {
+    if (a.mean) a.mean[row] = mean;
+    if (a.ivar) a.ivar[row] = ivar;
+  }
 }
 
-// sums over the rows first: the error may be written over delta
-template <class Rows>
-__global__ __launch_bounds__(THREADS) void ln_parameters_kernel(float *dgamma, float *dbeta, const float *delta, const float *gamma, const float *beta, Rows x,
-                                                                const float *mean, const float *ivar, size_t rows, uint32_t N, int func, bool accumulate) {
-  const uint32_t i = blockIdx.x * 64u + threadIdx.x % 64u, slice = threadIdx.x / 64u;
-  __shared__ float part[2][4][64];
-  float sg = 0.f, sb = 0.f;
-  if (i < N)
-    for (size_t row = slice; row < rows; row += 4) {
-      const float xhat = (x.at(row, i) - mean[row]) * ivar[row];
-      const float g = front(func, delta[row * N + i], gamma[i], xhat, beta, i);
-      sg += g * xhat;
-      sb += g;
+// longer rows: pieces of PIECE values, one block each.  First the mean and the sum of squared deviations of every piece ...
+constexpr uint32_t PIECE = 4096;
+template <bool VEC, bool PACK>
+__global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *stats, uint32_t pieces) {
+  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  __shared__ float part[2][THREADS / 64];
+  const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE);
+  float x[PIECE / THREADS];
+  S::load(x, a.in + (size_t)row * a.N + (size_t)piece * PIECE, n, 0.f);
+  if (PACK) {
+    const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N + piece * PIECE;
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++) pack_step(a.packed, w, e0 + S::first(j), S::first(j) < n, x + j * S::WIDTH);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < (int)(PIECE / THREADS); k++) s += x[k];
+  const float mean = row_sum<THREADS>(s, part[0]) / (float)n;
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++)
+#pragma unroll
+    for (int e = 0; e < S::WIDTH; e++) {
+      const float d = S::first(j) < n ? x[j * S::WIDTH + e] - mean : 0.f;
+      s += d * d;
     }
-  part[0][slice][threadIdx.x % 64] = sg;
-  part[1][slice][threadIdx.x % 64] = sb;
+  s = row_sum<THREADS>(s, part[1]);
+  if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, s);
+}
+// ... then every block joins the pieces of its row (each wavefront for itself: the sum of deviations of a piece moves by
+// n * (its mean - the row's mean)^2) and normalises its own piece
+template <bool VEC>
+__global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const float2 *stats, uint32_t pieces) {
+  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, lane = threadIdx.x % 64, n = min(PIECE, a.N - piece * PIECE);
+  const size_t at = (size_t)row * a.N + (size_t)piece * PIECE;
+  float x[PIECE / THREADS];
+  S::load(x, a.in + at, n, 0.f);
+  stats += (size_t)row * pieces;
+  float s = 0.f;
+  for (uint32_t p = lane; p < pieces; p += 64) s += stats[p].x * (float)min(PIECE, a.N - p * PIECE);
+  const float mean = over_lanes<Sum, 64>(s) / (float)a.N;
+  s = 0.f;
+  for (uint32_t p = lane; p < pieces; p += 64) {
+    const float2 t = stats[p];
+    const float d = t.x - mean;
+    s += t.y + d * d * (float)min(PIECE, a.N - p * PIECE);
+  }
+  const float ivar = 1.f / sqrtf(over_lanes<Sum, 64>(s) / (float)a.N + a.eps);
+  normalise<THREADS, PIECE / THREADS, VEC>(a, a.out + at, x, mean, ivar, a.gamma + (size_t)piece * PIECE, a.beta + (size_t)piece * PIECE, n);
+  if (piece == 0 && threadIdx.x == 0) {
+    if (a.mean) a.mean[row] = mean;
+    if (a.ivar) a.ivar[row] = ivar;
+  }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------
+struct Backward {
+  float *error;
+  float *dgamma, *dbeta;  // null: not wanted
+  const float *delta, *gamma, *beta, *mean, *ivar;
+  uint32_t rows, N;
+  int func;
+  bool accumulate;
+};
+
+// delta * f'(gamma * xhat + beta) for the functions that the kernels hold inline
+__device__ __forceinline__ float front(int func, float delta, float gamma, float xhat, float beta) {
+  const float pre = gamma * xhat + beta;
+  if (func == MT_F_RELU) return pre >= 0.f ? delta : delta * 0.f;
+  if (func == MT_F_LEAKY_RELU) return delta * (pre >= 0.f ? 1.f : 0.1f);
+  if (func == MT_F_SIGMOID) {
+    const float f = mt::f_sigmoid_fast(pre);
+    return delta * ((1.f - f) * f);
+  }
+  const float f = mt::f_tangence_fast(pre);
+  return delta * (1.f - f * f);
+}
+// xhat and the gradient in front of the function for one step of a row
+template <int WIDTH>
+__device__ __forceinline__ void step_terms(const Backward &a, float mean, float ivar, const float *gamma, uint32_t at, float *x, float *g) {
+#pragma unroll
+  for (int e = 0; e < WIDTH; e++) x[e] = (x[e] - mean) * ivar;
+  if (a.func != MT_F_NONE) {
+    float b[WIDTH];
+    load_step<WIDTH == 4>(b, a.beta, at);
+#pragma unroll
+    for (int e = 0; e < WIDTH; e++) g[e] = front(a.func, g[e], gamma[e], x[e], b[e]);
+  }
+}
+
+// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per block, four wavefronts that take
+// every fourth row, joined in a fixed order
+__global__ __launch_bounds__(THREADS) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N, bool accumulate) {
+  __shared__ float sums[4][64];
+  const uint32_t i = blockIdx.x * 64u + threadIdx.x % 64u, slice = threadIdx.x / 64u;
+  float *out = blockIdx.y == 0 ? dgamma : dbeta;
+  if (out == nullptr) return;
+  const float *p = partial + (size_t)blockIdx.y * parts * N + i;
+  float s = 0.f;
+  if (i < N) {
+    uint32_t k = slice;
+    for (; k + 28 < parts; k += 32) {
+      float t[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) t[u] = p[(size_t)(k + 4 * u) * N];
+      s += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+    }
+    for (; k < parts; k += 4) s += p[(size_t)k * N];
+  }
+  sums[slice][threadIdx.x % 64u] = s;
   __syncthreads();
   if (slice == 0 && i < N) {
     const uint32_t c = threadIdx.x;
-    sg = ((part[0][0][c] + part[0][1][c]) + part[0][2][c]) + part[0][3][c];
-    sb = ((part[1][0][c] + part[1][1][c]) + part[1][2][c]) + part[1][3][c];
-    if (dgamma) dgamma[i] = accumulate ? dgamma[i] + sg : sg;
-    if (dbeta) dbeta[i] = accumulate ? dbeta[i] + sb : sb;
+    s = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    out[i] = accumulate ? out[i] + s : s;
   }
 }
 
-template <class Rows>
-__global__ __launch_bounds__(THREADS) void ln_error_kernel(float *error, const float *delta, const float *gamma, const float *beta, Rows x, const float *mean,
-                                                           const float *ivar, size_t rows, uint32_t N, int func) {
-  __shared__ float part[THREADS / 64];
-  for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float m = mean[row], iv = ivar[row];
+// rows that fit the registers of L threads; a block walks over the rows and keeps its share of dgamma and dbeta in registers
+template <int L, int E, bool VEC, class Rows>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
+  using S = Share<L, E, VEC>;
+  constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
+  constexpr int W = S::WIDTH;
+  __shared__ float part[2][2][L / 64 + 1];
+  __shared__ float shared[L < 256 ? 2 * 256 * E : 1];
+  const uint32_t sub = threadIdx.x / L, lane = threadIdx.x % L;
+  float dg[E], db[E], gamma[E];
+  S::load(gamma, a.gamma, a.N, 0.f);
+#pragma unroll
+  for (int k = 0; k < E; k++) dg[k] = db[k] = 0.f;
+  uint32_t turn = 0;
+  for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += gridDim.x * PER_BLOCK, turn ^= 1u) {
+    const uint32_t row = min(first + sub, a.rows - 1);
+    const bool mine = first + sub < a.rows;
+    const float mean = a.mean[row], ivar = a.ivar[row];
+    const auto in = rows.row(row);
+    float x[E], g[E];
+    S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, min(S::first(j), a.N - W));
     float s1 = 0.f, s2 = 0.f;
-    for (uint32_t i = threadIdx.x; i < N; i += THREADS) {
-      const float xhat = (x.at(row, i) - m) * iv, u = front(func, delta[row * N + i], gamma[i], xhat, beta, i) * gamma[i];
-      s1 += u;
-      s2 += u * xhat;
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++) {
+      step_terms<W>(a, mean, ivar, gamma + j * W, min(S::first(j), a.N - W), x + j * W, g + j * W);
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        const int k = j * W + e;
+        if (S::first(j) >= a.N) x[k] = g[k] = 0.f;
+        if (mine) {
+          dg[k] += g[k] * x[k];
+          db[k] += g[k];
+        }
+        g[k] *= gamma[k];
+        s1 += g[k];
+        s2 += g[k] * x[k];
+      }
     }
-    s1 = block_sum(s1, part) / (float)N;
-    s2 = block_sum(s2, part) / (float)N;
-    for (uint32_t i = threadIdx.x; i < N; i += THREADS) {
-      const float xhat = (x.at(row, i) - m) * iv, u = front(func, delta[row * N + i], gamma[i], xhat, beta, i) * gamma[i];
-      error[row * N + i] = iv * ((u - s1) - xhat * s2);
+    // both sums with one barrier; the next row uses the other half of `part`
+    s1 = over_lanes<Sum, L < 64 ? L : 64>(s1);
+    s2 = over_lanes<Sum, L < 64 ? L : 64>(s2);
+    if (L > 64) {
+      if (threadIdx.x % 64 == 0) {
+        part[turn][0][threadIdx.x / 64] = s1;
+        part[turn][1][threadIdx.x / 64] = s2;
+      }
+      __syncthreads();
+      s1 = part[turn][0][0];
+      s2 = part[turn][1][0];
+#pragma unroll
+      for (int k = 1; k < L / 64; k++) {
+        s1 += part[turn][0][k];
+        s2 += part[turn][1][k];
+      }
+    }
+    s1 /= (float)a.N;
+    s2 /= (float)a.N;
+    float *error = a.error + (size_t)row * a.N;
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < S::STEPS; j++) {
+        if (S::first(j) >= a.N) continue;
+        float t[W];
+#pragma unroll
+        for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
+        S::store(error, j, t);
+      }
+    }
+  }
+  if (a.dgamma == nullptr && a.dbeta == nullptr) return;
+  float *pg = partial + (size_t)blockIdx.x * a.N, *pb = partial + ((size_t)gridDim.x + blockIdx.x) * a.N;
+  if (L >= 256) {
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++)
+      if (S::first(j) < a.N) {
+        S::store(pg, j, dg + j * W);
+        S::store(pb, j, db + j * W);
+      }
+    return;
+  }
+  // the block's rows of partial sums, joined in LDS: [of g * xhat, of g][row of the block][value]
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++)
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      shared[sub * (L * E) + S::first(j) + e] = dg[j * W + e];
+      shared[256 * E + sub * (L * E) + S::first(j) + e] = db[j * W + e];
+    }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < a.N; i += 256) {
+    float sg = 0.f, sb = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < PER_BLOCK; k++) {
+      sg += shared[k * (L * E) + i];
+      sb += shared[256 * E + k * (L * E) + i];
+    }
+    pg[i] = sg;
+    pb[i] = sb;
+  }
+  (void)lane;
+}
+
+// longer rows: the two sums of every piece ...
+template <bool VEC, class Rows>
+__global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a, Rows rows, float2 *sums, uint32_t pieces) {
+  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  constexpr int W = S::WIDTH;
+  __shared__ float part[2][THREADS / 64];
+  const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE), at = piece * PIECE;
+  const float mean = a.mean[row], ivar = a.ivar[row];
+  const auto in = rows.row(row);
+  float x[PIECE / THREADS], g[PIECE / THREADS];
+  S::load(g, a.delta + (size_t)row * a.N + at, n, 0.f);
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, at + min(S::first(j), n - W));
+  float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) {
+    const uint32_t i = at + min(S::first(j), n - W);
+    float gamma[W];
+    load_step<VEC>(gamma, a.gamma, i);
+    step_terms<W>(a, mean, ivar, gamma, i, x + j * W, g + j * W);
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      const float u = S::first(j) < n ? g[j * W + e] * gamma[e] : 0.f;
+      s1 += u;
+      s2 += S::first(j) < n ? u * x[j * W + e] : 0.f;
+    }
+  }
+  s1 = row_sum<THREADS>(s1, part[0]);
+  s2 = row_sum<THREADS>(s2, part[1]);
+  if (threadIdx.x == 0) sums[blockIdx.x] = make_float2(s1, s2);
+}
+// ... then blocks of 256 * WIDTH columns that walk over a group of rows: the error, and their columns' share of dgamma and dbeta
+constexpr uint32_t GROUP_ROWS = 64;  // rows of a group, at most
+template <bool VEC, class Rows>
+__global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a, Rows rows, const float2 *sums, uint32_t pieces, uint32_t groups, uint32_t per_group,
+                                                                     float *partial) {
+  constexpr int W = VEC ? 4 : 1;
+  __shared__ float4 terms[GROUP_ROWS];  // of each row: mean, ivar, sum(u) / N, sum(u * xhat) / N
+  const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * THREADS + threadIdx.x) * W, at = min(column, a.N - W);
+  const uint32_t first = group * per_group, count = min(per_group, a.rows - first), lane = threadIdx.x % 64;
+  for (uint32_t k = threadIdx.x / 64; k < count; k += THREADS / 64) {
+    const float2 *p = sums + (size_t)(first + k) * pieces;
+    float s1 = 0.f, s2 = 0.f;
+    for (uint32_t i = lane; i < pieces; i += 64) {
+      s1 += p[i].x;
+      s2 += p[i].y;
+    }
+    s1 = over_lanes<Sum, 64>(s1) / (float)a.N;
+    s2 = over_lanes<Sum, 64>(s2) / (float)a.N;
+    if (lane == 0) terms[k] = make_float4(a.mean[first + k], a.ivar[first + k], s1, s2);
+  }
+  float gamma[W], dg[W] = {}, db[W] = {};
+  load_step<VEC>(gamma, a.gamma, at);
+  __syncthreads();
+  // four rows at a time, loaded before the first of them is stored (the error may be written over delta: each thread reads and
+  // writes its own columns)
+  constexpr uint32_t AT_ONCE = 4;
+  for (uint32_t k0 = 0; k0 < count; k0 += AT_ONCE) {
+    float x[AT_ONCE][W], g[AT_ONCE][W];
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; u++) {
+      const uint32_t row = first + min(k0 + u, count - 1);
+      load_step<VEC>(g[u], a.delta + (size_t)row * a.N, at);
+      rows.row(row).template step<VEC>(x[u], at);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; u++) {
+      if (k0 + u >= count) break;
+      const float4 c = terms[k0 + u];
+      float t[W];
+      step_terms<W>(a, c.x, c.y, gamma, at, x[u], g[u]);
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        dg[e] += g[u][e] * x[u][e];
+        db[e] += g[u][e];
+        t[e] = c.y * ((g[u][e] * gamma[e] - c.z) - x[u][e] * c.w);
+      }
+      if (column < a.N) {
+        float *p = a.error + (size_t)(first + k0 + u) * a.N + column;
+        if (VEC)
+          *reinterpret_cast<float4 *>(p) = make_float4(t[0], t[W / 4], t[W / 2], t[W - 1]);
+        else
+          *p = t[0];
+      }
+    }
+  }
+  if (column >= a.N) return;
+  if (groups > 1) {
+    float *pg = partial + (size_t)group * a.N + column, *pb = partial + ((size_t)groups + group) * a.N + column;
+    if (a.dgamma || a.dbeta)
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        pg[e] = dg[e];
+        pb[e] = db[e];
+      }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < W; e++) {
+    if (a.dgamma) a.dgamma[column + e] = a.accumulate ? a.dgamma[column + e] + dg[e] : dg[e];
+    if (a.dbeta) a.dbeta[column + e] = a.accumulate ? a.dbeta[column + e] + db[e] : db[e];
+  }
+}
+
+// error = delta * f'(gamma * xhat + beta) alone, for a function that the kernels above do not hold (GeLU: double arithmetic and two
+// library functions); the backward pass then starts from it
+template <class Rows>
+__global__ __launch_bounds__(THREADS) void ln_front_kernel(Backward a, Rows rows) {
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float mean = a.mean[row], ivar = a.ivar[row];
+    const auto in = rows.row(row);
+    for (uint32_t i = blockIdx.y * THREADS + threadIdx.x; i < a.N; i += gridDim.y * THREADS) {
+      float x;
+      in.template step<false>(&x, i);
+      const size_t e = (size_t)row * a.N + i;
+      a.error[e] = a.delta[e] * mt::apply_func(MT_F_DIFFERENTIAL + a.func, a.gamma[i] * ((x - mean) * ivar) + a.beta[i]);
     }
   }
 }
+
+mt::Workspace g_ln_ws;
+int ln_workspace(size_t floats, float **p) { return mt::workspace_get(g_ln_ws, "layer-norm sums", floats, p); }
+
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 // ---- sizes ---------------------------------------------------------------------------------------------------------
 struct Geometry {
-  size_t rows;
-  uint32_t N, per_sample;   // values per row, rows per sample
+  uint32_t rows, N, per_sample;  // rows, values per row, rows per sample
   uint32_t kept_z, kept_y;  // sizes of a statistic: [W,kept_z,kept_y,1]
 };
 
@@ -134,9 +587,9 @@ int geometry(const char *name, const mt_tensor *in, const mt_tensor *gamma, Geom
   }
   const uint64_t per = (uint64_t)g->kept_z * g->kept_y, zy = (uint64_t)gamma->z * gamma->y;
   uint64_t N, rows;
-  if (__builtin_mul_overflow(zy, (uint64_t)gamma->x, &N) || N > 0x7fffffefull || per > 0x7fffffffull || __builtin_mul_overflow(per, (uint64_t)in->w, &rows) || rows >= (1ull << 40))
-    return mt::fail(MT_E_UNAVAILABLE, "%s: rows of 2^31 values or more are not supported", name);
-  g->rows = rows;
+  if (__builtin_mul_overflow(zy, (uint64_t)gamma->x, &N) || N > 0x7fffffefull || per > 0x7fffffffull || __builtin_mul_overflow(per, (uint64_t)in->w, &rows) || rows > 0x7fffffffull)
+    return mt::fail(MT_E_UNAVAILABLE, "%s: 2^31 rows, or rows of 2^31 values, are not supported", name);
+  g->rows = (uint32_t)rows;
   g->N = (uint32_t)N;
   g->per_sample = (uint32_t)per;
   return MT_OK;
@@ -144,18 +597,111 @@ int geometry(const char *name, const mt_tensor *in, const mt_tensor *gamma, Geom
 bool same_sizes(const mt_tensor *a, const mt_tensor *b) { return mt::same_zyx(a, b) && a->w == b->w; }
 bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { return t->w == in->w && t->z == g.kept_z && t->y == g.kept_y && t->x == 1; }
 
+// rows of up to this many values are held in registers
+constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384;
+
+template <int L, int E>
+void forward_rows(const Forward &a, bool vec, bool pack) {
+  const unsigned grid = cdiv(a.rows, L < 256 ? 256 / L : 1), threads = L < 256 ? 256 : L;
+  if constexpr (L >= 64) {
+    if (pack) {
+      ln_forward_kernel<L, E, true, true><<<grid, threads, 0, mt::stream()>>>(a);
+      return;
+    }
+  }
+  if (vec)
+    ln_forward_kernel<L, E, true, false><<<grid, threads, 0, mt::stream()>>>(a);
+  else
+    ln_forward_kernel<L, E, false, false><<<grid, threads, 0, mt::stream()>>>(a);
+}
+
+// calls f with the threads per row and the values per thread that hold a row of N values
+template <class F>
+int with_share(uint32_t N, F &&f) {
+  using std::integral_constant;
+#define MT_LN_SHARE(L, E) \
+  if (N <= L * E) return f(integral_constant<int, L>{}, integral_constant<int, E>{})
+  MT_LN_SHARE(8, 4);
+  MT_LN_SHARE(16, 8);
+  MT_LN_SHARE(64, 4);
+  MT_LN_SHARE(64, 8);
+  MT_LN_SHARE(64, 16);
+  MT_LN_SHARE(256, 8);
+  MT_LN_SHARE(256, 16);
+  MT_LN_SHARE(256, 32);
+  MT_LN_SHARE(1024, 16);
+#undef MT_LN_SHARE
+  return f(integral_constant<int, 1024>{}, integral_constant<int, 32>{});
+}
+
 template <class Rows>
 int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
-             const mt_tensor *beta, const Rows &x, const mt_tensor *mean, const mt_tensor *ivar, int func, int accumulate, const Geometry &g) {
+             const mt_tensor *beta, const Rows &x, bool x_aligned, const mt_tensor *mean, const mt_tensor *ivar, int func, int accumulate, const Geometry &g) {
   mt::ProfileScope prof(name);
-  const float *pb = beta ? beta->p : nullptr;
-  if (dgamma || dbeta) {
-    ln_parameters_kernel<<<cdiv(g.N, 64), THREADS, 0, mt::stream()>>>(dgamma ? dgamma->p : nullptr, dbeta ? dbeta->p : nullptr, delta->p, gamma->p, pb, x, mean->p, ivar->p,
-                                                                      g.rows, g.N, func, accumulate != 0);
+  Backward a{};
+  a.error = error->p; a.dgamma = dgamma ? dgamma->p : nullptr; a.dbeta = dbeta ? dbeta->p : nullptr;
+  a.delta = delta->p; a.gamma = gamma->p; a.beta = beta ? beta->p : nullptr; a.mean = mean->p; a.ivar = ivar->p;
+  a.rows = g.rows; a.N = g.N; a.func = func; a.accumulate = accumulate != 0;
+  if (func == MT_F_GELU) {
+    ln_front_kernel<<<dim3(g.rows < 4096 ? g.rows : 4096, g.N < 65536 ? 1 : 16), THREADS, 0, mt::stream()>>>(a, x);
+    MT_LAUNCH_CHECK(name);
+    a.delta = a.error;
+    a.func = MT_F_NONE;
+  }
+  const bool params = dgamma || dbeta;
+  const bool vec = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
+  uint32_t parts = 0;
+  float *partial = nullptr;
+  if (g.N <= BACKWARD_ROW) {
+    int rc = with_share(g.N, [&](auto l, auto e) {
+      constexpr int L = l, E = e;
+      if constexpr (L * E <= (int)BACKWARD_ROW) {
+        const uint32_t per_block = L < 256 ? 256 / L : 1, threads = L < 256 ? 256 : L;
+        parts = cdiv(g.rows, per_block);
+        if (parts > 512) parts = 512;
+        if (params) {
+          int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
+          if (rc) return rc;
+        }
+        if (vec)
+          ln_backward_kernel<L, E, true, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+        else
+          ln_backward_kernel<L, E, false, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+      }
+      return (int)MT_OK;
+    });
+    if (rc) return rc;
+    MT_LAUNCH_CHECK(name);
+  } else {
+    const uint32_t pieces = cdiv(g.N, PIECE), strips = cdiv(g.N, THREADS * (vec ? 4 : 1));
+    uint32_t groups = cdiv(1024, strips);
+    if (groups > g.rows) groups = g.rows;
+    uint32_t per_group = cdiv(g.rows, groups);
+    if (per_group > GROUP_ROWS) per_group = GROUP_ROWS;
+    groups = cdiv(g.rows, per_group);
+    if ((uint64_t)g.rows * pieces > 0x7fffffffull || (uint64_t)groups * strips > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
+    const size_t sums = 2 * (size_t)g.rows * pieces;
+    float *ws = nullptr;
+    int rc = ln_workspace(sums + (params && groups > 1 ? 2 * (size_t)groups * g.N : 0), &ws);
+    if (rc) return rc;
+    float2 *piece_sums = reinterpret_cast<float2 *>(ws);
+    partial = ws + sums;
+    parts = groups > 1 ? groups : 0;
+    if (vec) {
+      ln_backward_pieces_kernel<true><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
+      MT_LAUNCH_CHECK(name);
+      ln_backward_columns_kernel<true><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
+    } else {
+      ln_backward_pieces_kernel<false><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
+      MT_LAUNCH_CHECK(name);
+      ln_backward_columns_kernel<false><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
+    }
     MT_LAUNCH_CHECK(name);
   }
-  ln_error_kernel<<<(unsigned)(g.rows < 8192 ? g.rows : 8192), THREADS, 0, mt::stream()>>>(error->p, delta->p, gamma->p, pb, x, mean->p, ivar->p, g.rows, g.N, func);
-  MT_LAUNCH_CHECK(name);
+  if (params && parts) {
+    ln_join_kernel<<<dim3(cdiv(g.N, 64), 2), THREADS, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
+    MT_LAUNCH_CHECK(name);
+  }
   return MT_OK;
 }
 
@@ -223,12 +769,45 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
   }
   if (g.N == 0 || g.rows == 0) return MT_OK;
   for (auto t : {out, mean, ivar}) mt::note_write(t);
-  if (packed_input && (rc = mt_pack(packed_input, in))) return rc;
-  mt::ProfileScope prof(name);
-  ln_forward_kernel<<<(unsigned)(g.rows < 8192 ? g.rows : 8192), THREADS, 0, mt::stream()>>>(out->p, in->p, gamma->p, beta->p, mean ? mean->p : nullptr,
-                                                                                             ivar ? ivar->p : nullptr, g.rows, g.N, epsilon, func);
-  MT_LAUNCH_CHECK(name);
-  return MT_OK;
+  Forward a{};
+  a.out = out->p; a.in = in->p; a.gamma = gamma->p; a.beta = beta->p; a.mean = mean ? mean->p : nullptr; a.ivar = ivar ? ivar->p : nullptr;
+  a.packed = packed; a.rows = g.rows; a.N = g.N; a.per_sample = g.per_sample; a.eps = epsilon;
+  a.func = func == MT_F_GELU ? MT_F_NONE : func;  // GeLU (double arithmetic, a library function) runs over the output afterwards
+  const bool vec = g.N % 4 == 0 && aligned16(a.out) && aligned16(a.in) && aligned16(a.gamma) && aligned16(a.beta);
+  // the same pass can leave the 8 bits where a row starts at a group's first value and 32 lanes hold a group
+  const bool pack = packed_input && vec && g.N > 128 && (g.N % mt::PACK_GROUP == 0 || g.per_sample == 1);
+  if (packed_input && !pack && (rc = mt_pack(packed_input, in))) return rc;
+  if (packed_input) mt::note_write(packed.q, mt::packed_bytes(packed));
+  {
+    mt::ProfileScope prof(name);
+    if (g.N <= FORWARD_ROW) {
+      rc = with_share(g.N, [&](auto l, auto e) {
+        forward_rows<decltype(l)::value, decltype(e)::value>(a, vec, pack);
+        return (int)MT_OK;
+      });
+      MT_LAUNCH_CHECK(name);
+    } else {
+      const uint32_t pieces = cdiv(g.N, PIECE);
+      if ((uint64_t)g.rows * pieces > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
+      float *ws = nullptr;
+      if ((rc = ln_workspace(2 * (size_t)g.rows * pieces, &ws))) return rc;
+      float2 *stats = reinterpret_cast<float2 *>(ws);
+      const unsigned grid = g.rows * pieces;
+      if (pack)
+        ln_pieces_kernel<true, true><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      else if (vec)
+        ln_pieces_kernel<true, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      else
+        ln_pieces_kernel<false, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      MT_LAUNCH_CHECK(name);
+      if (vec)
+        ln_apply_kernel<true><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      else
+        ln_apply_kernel<false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      MT_LAUNCH_CHECK(name);
+    }
+  }
+  return func == MT_F_GELU ? mt_apply_func(out, out, func) : MT_OK;
 }
 
 int mt_layernorm_backward_func(const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
@@ -243,7 +822,7 @@ int mt_layernorm_backward_func(const mt_tensor *error, const mt_tensor *dgamma, 
     if (t && mt::overlap(t, input)) return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with the input", name);
   if (g.N == 0 || g.rows == 0) return backward_empty(dgamma, dbeta, accumulate);
   for (auto t : {error, dgamma, dbeta}) mt::note_write(t);
-  return backward(name, error, dgamma, dbeta, delta, gamma, beta, RowsF32{input->p, g.N}, mean, ivar, func, accumulate, g);
+  return backward(name, error, dgamma, dbeta, delta, gamma, beta, RowsF32{input->p, g.N}, aligned16(input->p), mean, ivar, func, accumulate, g);
 }
 
 int mt_layernorm_backward_packed_func(const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
@@ -261,7 +840,7 @@ int mt_layernorm_backward_packed_func(const mt_tensor *error, const mt_tensor *d
     if (t && mt::overlap(t, v)) return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with the input", name);
   if (g.N == 0 || g.rows == 0) return backward_empty(dgamma, dbeta, accumulate);
   for (auto t : {error, dgamma, dbeta}) mt::note_write(t);
-  return backward(name, error, dgamma, dbeta, delta, gamma, beta, RowsPacked{v, g.N, g.per_sample}, mean, ivar, func, accumulate, g);
+  return backward(name, error, dgamma, dbeta, delta, gamma, beta, RowsPacked{v, g.N, g.per_sample}, true, mean, ivar, func, accumulate, g);
 }
 
 }  // extern "C"

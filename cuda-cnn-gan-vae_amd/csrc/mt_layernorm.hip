@@ -19,40 +19,11 @@ using mt::PackedView;
 
 constexpr int THREADS = 256;
 
-// ---- sums over the lanes of a row (8, 16 or 64 lanes of a wavefront, or whole blocks); every lane gets the same bits ----------
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
-}
-struct Sum {
-  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
-};
-struct Lowest {
-  static __device__ __forceinline__ float of(float a, float b) { return mt::min_nan(a, b); }
-};
-struct Highest {
-  static __device__ __forceinline__ float of(float a, float b) { return mt::max_nan(a, b); }
-};
-template <class Op, int L>
-__device__ __forceinline__ float over_lanes(float v) {
-  v = Op::of(v, dpp<0xb1>(v));                  // neighbours
-  v = Op::of(v, dpp<0x4e>(v));                  // pairs of a quad
-  v = Op::of(v, dpp<0x141>(v));                 // quads of eight lanes
-  if (L > 8) v = Op::of(v, dpp<0x140>(v));      // halves of sixteen
-  if (L > 16) {
-    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  }
-  if (L > 32) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  }
-  return v;
-}
+// ---- sums over the threads of a row; every thread gets the same bits ----------------------------------------------------
 // over the L threads of a row; `part` (L / 64 values, rows of whole blocks) is used once: no second barrier
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float *part) {
-  v = over_lanes<Sum, L < 64 ? L : 64>(v);
+  v = mt::over_lanes<mt::Sum, L < 64 ? L : 64>(v);
   if (L > 64) {
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
     __syncthreads();
@@ -143,8 +114,8 @@ struct RowsPacked {
 // `valid` false; those behind the end of the sample write its padding
 __device__ __forceinline__ void pack_step(const PackedView &out, size_t sample, uint32_t e, bool valid, const float *t) {
   float low = mt::min_nan(mt::min_nan(t[0], t[1]), mt::min_nan(t[2], t[3])), high = mt::max_nan(mt::max_nan(t[0], t[1]), mt::max_nan(t[2], t[3]));
-  low = over_lanes<Lowest, 32>(valid ? low : __int_as_float(0x7f800000));
-  high = over_lanes<Highest, 32>(valid ? high : __int_as_float(0xff800000));
+  low = mt::over_lanes<mt::Lowest, 32>(valid ? low : __int_as_float(0x7f800000));
+  high = mt::over_lanes<mt::Highest, 32>(valid ? high : __int_as_float(0xff800000));
   const mt::PackScale s = mt::pack_scale(low, high);
   uint32_t w = 0;
 #pragma unroll
@@ -259,14 +230,14 @@ __global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const floa
   stats += (size_t)row * pieces;
   float s = 0.f;
   for (uint32_t p = lane; p < pieces; p += 64) s += stats[p].x * (float)min(PIECE, a.N - p * PIECE);
-  const float mean = over_lanes<Sum, 64>(s) / (float)a.N;
+  const float mean = mt::over_lanes<mt::Sum, 64>(s) / (float)a.N;
   s = 0.f;
   for (uint32_t p = lane; p < pieces; p += 64) {
     const float2 t = stats[p];
     const float d = t.x - mean;
     s += t.y + d * d * (float)min(PIECE, a.N - p * PIECE);
   }
-  const float ivar = 1.f / sqrtf(over_lanes<Sum, 64>(s) / (float)a.N + a.eps);
+  const float ivar = 1.f / sqrtf(mt::over_lanes<mt::Sum, 64>(s) / (float)a.N + a.eps);
   normalise<THREADS, PIECE / THREADS, VEC>(a, a.out + at, x, mean, ivar, a.gamma + (size_t)piece * PIECE, a.beta + (size_t)piece * PIECE, n);
   if (piece == 0 && threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
@@ -378,8 +349,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
       }
     }
     // both sums with one barrier; the next row uses the other half of `part`
-    s1 = over_lanes<Sum, L < 64 ? L : 64>(s1);
-    s2 = over_lanes<Sum, L < 64 ? L : 64>(s2);
+    s1 = mt::over_lanes<mt::Sum, L < 64 ? L : 64>(s1);
+    s2 = mt::over_lanes<mt::Sum, L < 64 ? L : 64>(s2);
     if (L > 64) {
       if (threadIdx.x % 64 == 0) {
         part[turn][0][threadIdx.x / 64] = s1;
@@ -488,8 +459,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
       s1 += p[i].x;
       s2 += p[i].y;
     }
-    s1 = over_lanes<Sum, 64>(s1) / (float)a.N;
-    s2 = over_lanes<Sum, 64>(s2) / (float)a.N;
+    s1 = mt::over_lanes<mt::Sum, 64>(s1) / (float)a.N;
+    s2 = mt::over_lanes<mt::Sum, 64>(s2) / (float)a.N;
     if (lane == 0) terms[k] = make_float4(a.mean[first + k], a.ivar[first + k], s1, s2);
   }
   float gamma[W], dg[W] = {}, db[W] = {};

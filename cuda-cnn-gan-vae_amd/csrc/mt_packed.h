@@ -89,4 +89,35 @@ __device__ __forceinline__ float unpack_value(float2 pair, uint32_t q) { return 
 __device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// sums, minima and maxima over 8, 16, 32 or 64 neighbouring lanes without LDS; every lane gets the same bits
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+struct Sum {
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct Lowest {
+  static __device__ __forceinline__ float of(float a, float b) { return min_nan(a, b); }
+};
+struct Highest {
+  static __device__ __forceinline__ float of(float a, float b) { return max_nan(a, b); }
+};
+template <class Op, int L>
+__device__ __forceinline__ float over_lanes(float v) {
+  v = Op::of(v, dpp<0xb1>(v));                  // neighbours
+  v = Op::of(v, dpp<0x4e>(v));                  // pairs of a quad
+  v = Op::of(v, dpp<0x141>(v));                 // quads of eight lanes
+  if (L > 8) v = Op::of(v, dpp<0x140>(v));      // halves of sixteen
+  if (L > 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  if (L > 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  return v;
+}
+
 }  // namespace mt

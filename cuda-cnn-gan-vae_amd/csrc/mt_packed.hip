@@ -1,53 +1,130 @@
 // Activations in 8 bits: mt_pack and mt_unpack.
+#include <type_traits>
+
 #include "mt_packed.h"
 
 namespace {
 
-using mt::cdiv;
 using mt::PackedView;
 
 constexpr int THREADS = 256;
+constexpr int LANES = 32;    // lanes that share a group: four values each
+constexpr int AT_ONCE = 4;   // groups in flight per 32 lanes
 
-inline unsigned blocks_for(size_t units, size_t per_block) {
-  const size_t b = (units + per_block - 1) / per_block;
-  return (unsigned)(b < 16384 ? b : 16384);
+// Both kernels move 5 bytes per value and compute little: what they need is enough loads in flight.  32 lanes take a group, four
+// values each (one 128-bit access where the tensor allows, four values 32 apart otherwise), and work on four groups at once.
+// Samples of whole groups are one long row of groups (`rows` false): no division by the groups of a sample is needed then.
+struct PackJob {
+  PackedView v;
+  uint64_t total;  // groups of the whole tensor
+  bool rows;
+};
+struct Place {
+  size_t tensor, bytes;  // where the group starts in the fp32 tensor and among the bytes
+  uint32_t count, room;  // its values, and its bytes with the sample's padding
+};
+template <class Index>
+__device__ __forceinline__ Place place(const PackJob &job, uint64_t g) {
+  if (!job.rows) return Place{(size_t)g * mt::PACK_GROUP, (size_t)g * mt::PACK_GROUP, mt::PACK_GROUP, mt::PACK_GROUP};
+  const Index w = (Index)g / job.v.groups;
+  const uint32_t first = (uint32_t)((Index)g - w * job.v.groups) * mt::PACK_GROUP;
+  return Place{(size_t)w * job.v.n + first, (size_t)w * job.v.pitch + first, min(mt::PACK_GROUP, job.v.n - first), min(mt::PACK_GROUP, job.v.pitch - first)};
 }
+// value k of a lane within its group, and whether a lane's four are next to each other
+template <bool VEC>
+__device__ __forceinline__ uint32_t within(uint32_t lane, int k) { return VEC ? lane * 4u + k : lane + 32u * k; }
 
-// 32 lanes per group, four elements 32 apart per lane
-__global__ __launch_bounds__(THREADS) void pack_kernel(PackedView out, const float *in, size_t total) {
-  const uint32_t lane = threadIdx.x & 31u;
-  for (size_t g = (size_t)blockIdx.x * (THREADS / 32) + threadIdx.x / 32; g < total; g += (size_t)gridDim.x * (THREADS / 32)) {
-    const size_t w = g / out.groups;
-    const uint32_t first = (uint32_t)(g - w * out.groups) * mt::PACK_GROUP;
-    const float *src = in + w * out.n;
-    float v[4], low, high;
+template <bool VEC, class Index>
+__global__ __launch_bounds__(THREADS) void pack_kernel(PackJob job, const float *in) {
+  const uint32_t lane = threadIdx.x % LANES;
+  const uint64_t step = (uint64_t)gridDim.x * (THREADS / LANES);
+  for (uint64_t g0 = (uint64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES; g0 < job.total; g0 += AT_ONCE * step) {
+    Place at[AT_ONCE];
+    float v[AT_ONCE][4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint32_t i = first + lane + 32u * k;
-      v[k] = src[i < out.n ? i : first];  // behind the end: a value of the group again
-      low = k ? mt::min_nan(low, v[k]) : v[k];
-      high = k ? mt::max_nan(high, v[k]) : v[k];
+    for (int u = 0; u < AT_ONCE; u++) {
+      const uint64_t g = g0 + u * step < job.total ? g0 + u * step : g0;
+      at[u] = place<Index>(job, g);
+      if (VEC) {
+        const float4 t = *reinterpret_cast<const float4 *>(in + at[u].tensor + min(lane * 4u, at[u].count - 4u));  // behind the end: values of the group again
+        v[u][0] = t.x; v[u][1] = t.y; v[u][2] = t.z; v[u][3] = t.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[u][k] = in[at[u].tensor + min(within<VEC>(lane, k), at[u].count - 1u)];
+      }
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      low = mt::min_nan(low, __shfl_xor(low, off, 64));
-      high = mt::max_nan(high, __shfl_xor(high, off, 64));
-    }
-    const mt::PackScale s = mt::pack_scale(low, high);
-    if (lane == 0) out.pair[g] = make_float2(s.low, s.step);
+    for (int u = 0; u < AT_ONCE; u++) {
+      if (g0 + u * step >= job.total) return;
+      const float low = mt::over_lanes<mt::Lowest, LANES>(mt::min_nan(mt::min_nan(v[u][0], v[u][1]), mt::min_nan(v[u][2], v[u][3])));
+      const float high = mt::over_lanes<mt::Highest, LANES>(mt::max_nan(mt::max_nan(v[u][0], v[u][1]), mt::max_nan(v[u][2], v[u][3])));
+      const mt::PackScale s = mt::pack_scale(low, high);
+      if (lane == 0) job.v.pair[g0 + u * step] = make_float2(s.low, s.step);
+      uint32_t q[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint32_t i = first + lane + 32u * k;
-      if (i < out.pitch) out.q[w * out.pitch + i] = i < out.n ? (uint8_t)mt::pack_value(s, v[k]) : (uint8_t)0;
+      for (int k = 0; k < 4; k++) q[k] = within<VEC>(lane, k) < at[u].count ? mt::pack_value(s, v[u][k]) : 0u;
+      uint8_t *p = job.v.q + at[u].bytes;
+      if (VEC) {
+        if (lane * 4u < at[u].room) *reinterpret_cast<uint32_t *>(p + lane * 4u) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (within<VEC>(lane, k) < at[u].room) p[within<VEC>(lane, k)] = (uint8_t)q[k];
+      }
     }
   }
 }
 
-__global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackedView in, size_t total) {
-  for (size_t e = (size_t)blockIdx.x * THREADS + threadIdx.x; e < total; e += (size_t)gridDim.x * THREADS) {
-    const size_t w = e / in.n;
-    const uint32_t i = (uint32_t)(e - w * in.n);
-    out[e] = mt::unpack_value(in.pair[w * in.groups + i / mt::PACK_GROUP], in.q[w * in.pitch + i]);
+template <bool VEC, class Index>
+__global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackJob job) {
+  const uint32_t lane = threadIdx.x % LANES;
+  const uint64_t step = (uint64_t)gridDim.x * (THREADS / LANES);
+  for (uint64_t g0 = (uint64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES; g0 < job.total; g0 += AT_ONCE * step) {
+    Place at[AT_ONCE];
+    float2 pair[AT_ONCE];
+    uint32_t q[AT_ONCE][4];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; u++) {
+      const uint64_t g = g0 + u * step < job.total ? g0 + u * step : g0;
+      at[u] = place<Index>(job, g);
+      pair[u] = job.v.pair[g];
+      const uint8_t *p = job.v.q + at[u].bytes;
+      if (VEC) {
+        q[u][0] = *reinterpret_cast<const uint32_t *>(p + min(lane * 4u, at[u].count - 4u));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[u][k] = p[min(within<VEC>(lane, k), at[u].count - 1u)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; u++) {
+      if (g0 + u * step >= job.total) return;
+      float *p = out + at[u].tensor;
+      if (VEC) {
+        float t[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) t[k] = mt::unpack_value(pair[u], (q[u][0] >> (8 * k)) & 255u);
+        if (lane * 4u < at[u].count) *reinterpret_cast<float4 *>(p + lane * 4u) = make_float4(t[0], t[1], t[2], t[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (within<VEC>(lane, k) < at[u].count) p[within<VEC>(lane, k)] = mt::unpack_value(pair[u], q[u][k]);
+      }
+    }
+  }
+}
+
+// calls f with the job, whether a lane's four values are one access, and the width that a group's number needs
+template <class F>
+void with_job(const PackedView &v, const float *tensor, F &&f) {
+  PackJob job{v, (uint64_t)v.w * v.groups, v.n % mt::PACK_GROUP != 0};
+  const uint64_t blocks = (job.total + THREADS / LANES * AT_ONCE - 1) / (THREADS / LANES * AT_ONCE);
+  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+  const bool vec = v.n % 4 == 0 && ((uintptr_t)tensor & 15u) == 0;
+  if (job.rows && job.total > 0xffffffffull) {
+    if (vec) f(job, grid, std::true_type{}, uint64_t{}); else f(job, grid, std::false_type{}, uint64_t{});
+  } else {
+    if (vec) f(job, grid, std::true_type{}, uint32_t{}); else f(job, grid, std::false_type{}, uint32_t{});
   }
 }
 
@@ -73,8 +150,9 @@ int mt_pack(const mt_packed_tensor *out, const mt_tensor *in) {
   if (mt::overlap(in, v)) return mt::fail(MT_E_ARGUMENT, "mt_pack: the packed tensor shares memory with the input");
   mt::note_write(v.q, mt::packed_bytes(v));
   mt::ProfileScope prof("mt_pack");
-  const size_t total = (size_t)v.w * v.groups;
-  pack_kernel<<<blocks_for(total, THREADS / 32), THREADS, 0, mt::stream()>>>(v, in->p, total);
+  with_job(v, in->p, [&](const PackJob &job, unsigned grid, auto vec, auto index) {
+    pack_kernel<decltype(vec)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(job, in->p);
+  });
   MT_LAUNCH_CHECK("mt_pack");
   return MT_OK;
 }
@@ -88,8 +166,9 @@ int mt_unpack(const mt_tensor *out, const mt_packed_tensor *in) {
   if (mt::overlap(out, v)) return mt::fail(MT_E_ARGUMENT, "mt_unpack: the packed tensor shares memory with the output");
   mt::note_write(out);
   mt::ProfileScope prof("mt_unpack");
-  const size_t total = (size_t)v.w * v.n;
-  unpack_kernel<<<blocks_for(total, THREADS), THREADS, 0, mt::stream()>>>(out->p, v, total);
+  with_job(v, out->p, [&](const PackJob &job, unsigned grid, auto vec, auto index) {
+    unpack_kernel<decltype(vec)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(out->p, job);
+  });
   MT_LAUNCH_CHECK("mt_unpack");
   return MT_OK;
 }

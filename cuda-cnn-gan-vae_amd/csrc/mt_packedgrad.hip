@@ -113,6 +113,7 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
   for (uint32_t s = 0; s < steps; s++) {
     const uint32_t buf = s & 1u, k = k0 + s * KSTEP;
     load_cols(k + KSTEP);
+    float offset[TM] = {}, bias[TM] = {};  // of this step: sums of sums keep their error at the root of 32 and of the steps
 #pragma unroll
     for (int kk = 0; kk < 4; kk++) {
       bf16x8 col[4];
@@ -128,8 +129,8 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
           for (int e = 0; e < 2; e++) {
             const float v = d[2 * j + e][m];
             const float2 sc = scale[buf][kk * 16 + half * 8u + 2 * j + e];
-            if (BIAS) sums.bias[m] += v;
-            sums.offset[m] = __builtin_fmaf(v, sc.y, sums.offset[m]);
+            if (BIAS) bias[m] += v;
+            offset[m] = __builtin_fmaf(v, sc.y, offset[m]);
             x[e] = v * sc.x;
             y[e] = x[e] - cut(x[e]);
             z[e] = y[e] - cut(y[e]);
@@ -139,8 +140,8 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
           cuts[2][j] = upper_halves(z[0], z[1]);
         }
         // (the compiler would leave these sums for the end of the step and keep four times the registers of delta for them)
-        asm volatile("" : "+v"(sums.offset[m]));
-        if (BIAS) asm volatile("" : "+v"(sums.bias[m]));
+        asm volatile("" : "+v"(offset[m]));
+        if (BIAS) asm volatile("" : "+v"(bias[m]));
         if (m == TM - 1) load_delta(k + 16u * (kk + 1));
 #pragma unroll
         for (int p = 0; p < 3; p++)
@@ -149,6 +150,11 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
             sums.acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, cuts[p]), col[n], sums.acc[m][n], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);  // nothing of the next 16 samples moves up: the registers are full
+    }
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      sums.offset[m] += offset[m];
+      if (BIAS) sums.bias[m] += bias[m];
     }
     store_cols(buf ^ 1u);
     __syncthreads();

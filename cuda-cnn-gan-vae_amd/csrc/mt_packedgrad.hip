@@ -32,7 +32,7 @@ typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // the next rows of an operand, at most `most` of the `left` that there are (none: left <= 0): what lies behind them reads as
-// zero.  most * row_bytes <= 2^31: 16 rows of delta, 64 of the packed bytes, fewer than 2^25 features.
+// zero.  most * row_bytes <= 2^30: 16 rows of delta or dweight, 64 of the packed bytes, fewer than 2^24 features.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void *p, int left, int most, uint32_t row_bytes) {
   const uint32_t rows = __builtin_amdgcn_readfirstlane(max(0, min(left, most)));  // (a clamp is a vector instruction: back to a scalar)
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)(rows * row_bytes), 0x00020000);
@@ -57,18 +57,22 @@ struct WgradSums {
   float offset[TM], bias[TM];    // the second sum and the sum of delta: row lane % 32, half of the samples each
 };
 
-// the product over the samples k0 ... k1; BIAS: the sum of delta too (the blocks of the first group)
-template <int TM, bool BIAS>
+// the product over the samples k0 ... k1.  The sum of delta is taken by all blocks though only those of the first group need it:
+// one addition in ten, where a second copy of the loop made those blocks the last ones (and the kernel's code twice as long).
+template <int TM>
 __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g, uint32_t m0, uint32_t k0, uint32_t k1, uintx4 (*cols)[KSTEP / 8][128], float2 (*scale)[KSTEP],
                                                   WgradSums<TM> &sums) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 31u, half = lane >> 5;
   const uint32_t steps = (k1 - k0 + KSTEP - 1) / KSTEP;
-  float d[8][TM];  // this lane's rows r * TM ... of eight samples
+  // this lane's rows r * TM ... of eight samples, AHEAD times 16 samples ahead of the products: 16 where two row tiles fill the
+  // registers (two wavefronts per SIMD hide the rest), a whole step where there is room and often one wavefront
+  constexpr int AHEAD = TM == 1 ? 4 : 1;
+  float d[AHEAD][8][TM];
   uint32_t voff[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) voff[j] = ((half * 8u + j) * a.Out + m0 + r * TM) * 4u;
 
-  auto load_delta = [&](uint32_t k) {
+  auto load_delta = [&](uint32_t k, float (&d)[8][TM]) {
     const auto rsrc = rows_rsrc(a.delta + (size_t)k * a.Out, (int)k1 - (int)k, 16, a.Out * 4u);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -107,7 +111,8 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
   };
 
   load_cols(k0);
-  load_delta(k0);
+#pragma unroll
+  for (int u = 0; u < AHEAD; u++) load_delta(k0 + 16u * u, d[u]);
   store_cols(0);
   __syncthreads();
   for (uint32_t s = 0; s < steps; s++) {
@@ -127,9 +132,9 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
           float x[2], y[2], z[2];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float v = d[2 * j + e][m];
+            const float v = d[kk % AHEAD][2 * j + e][m];
             const float2 sc = scale[buf][kk * 16 + half * 8u + 2 * j + e];
-            if (BIAS) bias[m] += v;
+            bias[m] += v;
             offset[m] = __builtin_fmaf(v, sc.y, offset[m]);
             x[e] = v * sc.x;
             y[e] = x[e] - cut(x[e]);
@@ -141,8 +146,8 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
         }
         // (the compiler would leave these sums for the end of the step and keep four times the registers of delta for them)
         asm volatile("" : "+v"(offset[m]));
-        if (BIAS) asm volatile("" : "+v"(bias[m]));
-        if (m == TM - 1) load_delta(k + 16u * (kk + 1));
+        asm volatile("" : "+v"(bias[m]));
+        if (m == TM - 1) load_delta(k + 16u * (kk + AHEAD), d[kk % AHEAD]);
 #pragma unroll
         for (int p = 0; p < 3; p++)
 #pragma unroll
@@ -154,7 +159,7 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
 #pragma unroll
     for (int m = 0; m < TM; m++) {
       sums.offset[m] += offset[m];
-      if (BIAS) sums.bias[m] += bias[m];
+      sums.bias[m] += bias[m];
     }
     store_cols(buf ^ 1u);
     __syncthreads();
@@ -165,6 +170,7 @@ template <int TM>
 __global__ __launch_bounds__(THREADS, 2) void packed_wgrad_kernel(WgradArgs a) {
   __shared__ uintx4 cols[2][KSTEP / 8][128];  // [eight samples][column]
   __shared__ float2 scale[2][KSTEP];          // (step, low + 128 * step)
+  __shared__ float4 offsets[4][TM][8];        // the second sum of every row of a wavefront
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, r = lane & 31u, half = lane >> 5;
   // neighbouring blocks of an XCD share their rows of delta (the larger operand) and walk over the groups
   uint32_t t = __builtin_amdgcn_readfirstlane(xcd_swizzle(blockIdx.x, gridDim.x));
@@ -180,38 +186,53 @@ __global__ __launch_bounds__(THREADS, 2) void packed_wgrad_kernel(WgradArgs a) {
 #pragma unroll
     for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
   }
-  if (bias)
-    packed_wgrad_loop<TM, true>(a, g, m0, k0, k1, cols, scale, sums);
-  else
-    packed_wgrad_loop<TM, false>(a, g, m0, k0, k1, cols, scale, sums);
+  packed_wgrad_loop<TM>(a, g, m0, k0, k1, cols, scale, sums);
 
   float *dw = a.dweight, *db = a.dbias;
   if (a.split > 1) {
     dw += (size_t)part * a.Out * a.in.n;
-    if (db) db += (size_t)part * a.Out;
+    if (bias) db += (size_t)part * a.Out;
   }
 #pragma unroll
   for (int m = 0; m < TM; m++) {
-    sums.offset[m] += __shfl_xor(sums.offset[m], 32, 64);
-    sums.bias[m] += __shfl_xor(sums.bias[m], 32, 64);
+    const float c = sums.offset[m] + __shfl_xor(sums.offset[m], 32, 64), sum = sums.bias[m] + __shfl_xor(sums.bias[m], 32, 64);
+    if (half == 0) reinterpret_cast<float *>(offsets[wave][m])[r] = c;
     if (bias && half == 0 && m0 + r * TM + m < a.Out) {
       float *p = db + m0 + r * TM + m;
-      *p = a.accumulate ? *p + sums.bias[m] : sums.bias[m];
+      *p = a.accumulate ? *p + sum : sum;
     }
+  }
+  __syncthreads();
+  // accumulator i of tile (m, n): row 8 * (i / 4) + 4 * half + i % 4, column 32 * n + r.  Rows and columns that do not exist have
+  // offsets behind the end of the buffer: their stores are dropped
+  const uint32_t row_bytes = a.in.n * 4u;
+  uint32_t voff[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const uint32_t row = 8u * (i / 4) + 4u * half + i % 4, o = m0 + row * TM + m;
-      const float c = __shfl(sums.offset[m], (int)row, 64);
-      if (o < a.Out)
+  for (int n = 0; n < 4; n++) {
+    const uint32_t c = g * 128u + n * 32u + r;
+    voff[n] = c < a.in.n ? 4u * half * TM * row_bytes + c * 4u : 0x80000000u;
+  }
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          const uint32_t col = g * 128u + n * 32u + r;
-          if (col < a.in.n) {
-            float *p = dw + (size_t)o * a.in.n + col;
-            const float v = sums.acc[m][n][i] + c;
-            *p = a.accumulate ? *p + v : v;
-          }
+  for (int i4 = 0; i4 < 4; i4++) {
+    const uint32_t o0 = __builtin_amdgcn_readfirstlane(m0 + 8u * i4 * TM);
+    const auto rsrc = rows_rsrc(dw + (size_t)o0 * a.in.n, (int)a.Out - (int)o0, 8 * TM, row_bytes);
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      const float4 c4 = offsets[wave][m][i4 * 2 + half];
+      const float c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t row = (i * TM + m) * row_bytes;
+        float v[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) v[n] = sums.acc[m][n][i4 * 4 + i] + c[i];
+        if (a.accumulate) {
+#pragma unroll
+          for (int n = 0; n < 4; n++) v[n] += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(voff[n] + row), 0, 0));
         }
+#pragma unroll
+        for (int n = 0; n < 4; n++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[n]), rsrc, (int)(voff[n] + row), 0, 0);
+      }
     }
   }
 }
@@ -256,8 +277,8 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   if (dweight->w != 1 || dweight->z != 1 || dweight->x != v.n || dweight->y != out || delta->w != v.w)
     return mt::fail(MT_E_SHAPE, "%s: dweight must be [1,1,Out,In], the input [B,...] of In values, delta [B,...] of Out values", name);
   if (dbias && (dbias->w != 1 || dbias->z != 1 || dbias->x != 1 || dbias->y != out)) return mt::fail(MT_E_SHAPE, "%s: dbias must be [1,1,Out,1]", name);
-  // a step's 64 samples are addressed with 32-bit offsets
-  if (v.n >= (1u << 25) || out >= (1u << 25)) return mt::fail(MT_E_UNAVAILABLE, "%s: 2^25 features or more are not supported", name);
+  // the rows of a step are addressed with 32-bit offsets
+  if (v.n >= (1u << 24) || out >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: 2^24 features or more are not supported", name);
   const uint32_t Out = (uint32_t)out;
   if (Out == 0) return MT_OK;
   for (auto t : {dweight, dbias})

@@ -119,7 +119,7 @@ __device__ __forceinline__ void pack_step(const PackedView &out, size_t sample, 
   const mt::PackScale s = mt::pack_scale(low, high);
   uint32_t w = 0;
 #pragma unroll
-  for (int k = 0; k < 4; k++) w |= mt::pack_value(s, t[k]) << (8 * k);
+  for (int k = 0; k < 4; k++) w = mt::pack_into(s, t[k], k, w);
   if (valid || (e >= out.n && e < out.pitch)) *reinterpret_cast<uint32_t *>(out.q + sample * out.pitch + e) = valid ? w : 0u;
   if (valid && e % mt::PACK_GROUP == 0) out.pair[sample * out.groups + e / mt::PACK_GROUP] = make_float2(s.low, s.step);
 }
@@ -280,30 +280,31 @@ __device__ __forceinline__ void step_terms(const Backward &a, float mean, float 
   }
 }
 
-// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per block, four wavefronts that take
-// every fourth row, joined in a fixed order
-__global__ __launch_bounds__(THREADS) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N, bool accumulate) {
-  __shared__ float sums[4][64];
+// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per block, sixteen wavefronts that take
+// every sixteenth row with eight loads in flight, joined in a fixed order (four wavefronts took 7.4 us for 512 rows of 2000, mostly
+// waiting for one batch of loads after the other)
+constexpr int JOIN_SLICES = 16;
+__global__ __launch_bounds__(64 * JOIN_SLICES) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N, bool accumulate) {
+  __shared__ float sums[JOIN_SLICES][64];
   const uint32_t i = blockIdx.x * 64u + threadIdx.x % 64u, slice = threadIdx.x / 64u;
   float *out = blockIdx.y == 0 ? dgamma : dbeta;
   if (out == nullptr) return;
-  const float *p = partial + (size_t)blockIdx.y * parts * N + i;
+  const float *p = partial + (size_t)blockIdx.y * parts * N + min(i, N - 1);
   float s = 0.f;
-  if (i < N) {
-    uint32_t k = slice;
-    for (; k + 28 < parts; k += 32) {
-      float t[8];
+  for (uint32_t k = slice; k < parts; k += 8 * JOIN_SLICES) {
+    float t[8];
 #pragma unroll
-      for (int u = 0; u < 8; u++) t[u] = p[(size_t)(k + 4 * u) * N];
-      s += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-    }
-    for (; k < parts; k += 4) s += p[(size_t)k * N];
+    for (int u = 0; u < 8; u++) t[u] = p[(size_t)min(k + u * JOIN_SLICES, parts - 1) * N];
+#pragma unroll
+    for (int u = 0; u < 8; u++) t[u] = k + u * JOIN_SLICES < parts ? t[u] : 0.f;
+    s += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   }
   sums[slice][threadIdx.x % 64u] = s;
   __syncthreads();
   if (slice == 0 && i < N) {
-    const uint32_t c = threadIdx.x;
-    s = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < JOIN_SLICES; k += 4) s += (sums[k][threadIdx.x] + sums[k + 1][threadIdx.x]) + (sums[k + 2][threadIdx.x] + sums[k + 3][threadIdx.x]);
     out[i] = accumulate ? out[i] + s : s;
   }
 }
@@ -599,7 +600,7 @@ int with_share(uint32_t N, F &&f) {
   MT_LN_SHARE(64, 16);
   MT_LN_SHARE(256, 8);
   MT_LN_SHARE(256, 16);
-  MT_LN_SHARE(256, 32);
+  MT_LN_SHARE(512, 16);
   MT_LN_SHARE(1024, 16);
 #undef MT_LN_SHARE
   return f(integral_constant<int, 1024>{}, integral_constant<int, 32>{});
@@ -645,8 +646,10 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     MT_LAUNCH_CHECK(name);
   } else {
     const uint32_t pieces = cdiv(g.N, PIECE), strips = cdiv(g.N, THREADS * (vec ? 4 : 1));
-    uint32_t groups = cdiv(1024, strips);
-    if (groups > g.rows) groups = g.rows;
+    // blocks that walk over all rows (at most 64) where the strips alone are three for four compute units: no partial sums to
+    // write and join.  Shorter rows: groups of at least 16 rows, so that the partial sums stay a twentieth of the traffic
+    uint32_t groups = strips >= 192 ? 1 : cdiv(1024, strips);
+    if (groups > cdiv(g.rows, 16)) groups = cdiv(g.rows, 16);
     uint32_t per_group = cdiv(g.rows, groups);
     if (per_group > GROUP_ROWS) per_group = GROUP_ROWS;
     groups = cdiv(g.rows, per_group);
@@ -670,7 +673,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     MT_LAUNCH_CHECK(name);
   }
   if (params && parts) {
-    ln_join_kernel<<<dim3(cdiv(g.N, 64), 2), THREADS, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
+    ln_join_kernel<<<dim3(cdiv(g.N, 64), 2), 64 * JOIN_SLICES, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
     MT_LAUNCH_CHECK(name);
   }
   return MT_OK;

@@ -76,13 +76,15 @@ __device__ __forceinline__ PackScale pack_scale(float low, float high) {
   s.step = finite ? range * (1.f / 255.f) : 0.f;
   if (s.step < FLT_MIN) s.step = 0.f;
   s.low = finite ? low : __int_as_float(0x7fc00000);
-  s.inverse = s.step > 0.f ? 1.f / s.step : 0.f;
+  // 1 / step, correctly rounded: the hardware's reciprocal and one step of Newton's method give the rounded quotient for every
+  // mantissa (all 2^23 compared with the division at ten exponents), without the scaling that a division does for
+  // subnormal numbers
+  const float r = __builtin_amdgcn_rcpf(s.step);
+  s.inverse = s.step > 0.f ? __builtin_fmaf(__builtin_fmaf(-s.step, r, 1.f), r, r) : 0.f;
   return s;
 }
-__device__ __forceinline__ uint32_t pack_value(const PackScale &s, float x) {
-  const float t = fminf(rintf((x - s.low) * s.inverse), 255.f);  // half to even; a NaN low gives 255, which its group never shows
-  return (uint32_t)t;
-}
+// the count of steps put into byte k of w: the instruction rounds half to even and holds the result within 0..255
+__device__ __forceinline__ uint32_t pack_into(const PackScale &s, float x, int k, uint32_t w) { return __builtin_amdgcn_cvt_pk_u8_f32((x - s.low) * s.inverse, k, w); }
 __device__ __forceinline__ float unpack_value(float2 pair, uint32_t q) { return pair.x + pair.y * (float)q; }
 
 // minimum and maximum that let a NaN through

@@ -60,16 +60,16 @@ __global__ __launch_bounds__(THREADS) void pack_kernel(PackJob job, const float 
       const float high = mt::over_lanes<mt::Highest, LANES>(mt::max_nan(mt::max_nan(v[u][0], v[u][1]), mt::max_nan(v[u][2], v[u][3])));
       const mt::PackScale s = mt::pack_scale(low, high);
       if (lane == 0) job.v.pair[g0 + u * step] = make_float2(s.low, s.step);
-      uint32_t q[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) q[k] = within<VEC>(lane, k) < at[u].count ? mt::pack_value(s, v[u][k]) : 0u;
       uint8_t *p = job.v.q + at[u].bytes;
       if (VEC) {
-        if (lane * 4u < at[u].room) *reinterpret_cast<uint32_t *>(p + lane * 4u) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+        uint32_t w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w = mt::pack_into(s, v[u][k], k, w);
+        if (lane * 4u < at[u].room) *reinterpret_cast<uint32_t *>(p + lane * 4u) = lane * 4u < at[u].count ? w : 0u;
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
-          if (within<VEC>(lane, k) < at[u].room) p[within<VEC>(lane, k)] = (uint8_t)q[k];
+          if (within<VEC>(lane, k) < at[u].room) p[within<VEC>(lane, k)] = within<VEC>(lane, k) < at[u].count ? (uint8_t)mt::pack_into(s, v[u][k], 0, 0u) : (uint8_t)0;
       }
     }
   }

@@ -280,33 +280,37 @@ __device__ __forceinline__ void step_terms(const Backward &a, float mean, float 
   }
 }
 
-// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per block, sixteen wavefronts that take
-// every sixteenth row with eight loads in flight, joined in a fixed order (four wavefronts took 7.4 us for 512 rows of 2000, mostly
-// waiting for one batch of loads after the other)
-constexpr int JOIN_SLICES = 16;
-__global__ __launch_bounds__(64 * JOIN_SLICES) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N, bool accumulate) {
-  __shared__ float sums[JOIN_SLICES][64];
-  const uint32_t i = blockIdx.x * 64u + threadIdx.x % 64u, slice = threadIdx.x / 64u;
+// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per SLICES wavefronts, which take every
+// SLICES-th row with eight loads in flight, joined in a fixed order.  Many parts: sixteen wavefronts (four took 7.4 us for 512 rows of
+// 2000, waiting for one batch of loads after the other; sixteen take 3).  Few parts of long rows: one (sixteen took 14 us for
+// 8 rows of 147456).
+constexpr uint32_t JOIN_MANY = 16;
+template <int SLICES>
+__global__ __launch_bounds__(SLICES == 1 ? THREADS : 64 * SLICES) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N,
+                                                                                     bool accumulate) {
+  constexpr uint32_t COLUMNS = SLICES == 1 ? THREADS : 64;
+  __shared__ float sums[SLICES][COLUMNS];
+  const uint32_t i = blockIdx.x * COLUMNS + threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS;
   float *out = blockIdx.y == 0 ? dgamma : dbeta;
   if (out == nullptr) return;
   const float *p = partial + (size_t)blockIdx.y * parts * N + min(i, N - 1);
   float s = 0.f;
-  for (uint32_t k = slice; k < parts; k += 8 * JOIN_SLICES) {
+  for (uint32_t k = slice; k < parts; k += 8 * SLICES) {
     float t[8];
 #pragma unroll
-    for (int u = 0; u < 8; u++) t[u] = p[(size_t)min(k + u * JOIN_SLICES, parts - 1) * N];
-#pragma unroll
-    for (int u = 0; u < 8; u++) t[u] = k + u * JOIN_SLICES < parts ? t[u] : 0.f;
+    for (int u = 0; u < 8; u++) t[u] = k + u * SLICES < parts ? p[(size_t)(k + u * SLICES) * N] : 0.f;
     s += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   }
-  sums[slice][threadIdx.x % 64u] = s;
-  __syncthreads();
-  if (slice == 0 && i < N) {
+  if (SLICES > 1) {
+    sums[slice][threadIdx.x % COLUMNS] = s;
+    __syncthreads();
+    if (slice != 0) return;
     s = 0.f;
 #pragma unroll
-    for (int k = 0; k < JOIN_SLICES; k += 4) s += (sums[k][threadIdx.x] + sums[k + 1][threadIdx.x]) + (sums[k + 2][threadIdx.x] + sums[k + 3][threadIdx.x]);
-    out[i] = accumulate ? out[i] + s : s;
+    for (int k = 0; k < SLICES; k += 4)
+      s += (sums[k][threadIdx.x] + sums[k + 1 < SLICES ? k + 1 : 0][threadIdx.x]) + (sums[k + 2 < SLICES ? k + 2 : 0][threadIdx.x] + sums[k + 3 < SLICES ? k + 3 : 0][threadIdx.x]);
   }
+  if (i < N) out[i] = accumulate ? out[i] + s : s;
 }
 
 // rows that fit the registers of L threads; a block walks over the rows and keeps its share of dgamma and dbeta in registers
@@ -323,15 +327,29 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 #pragma unroll
   for (int k = 0; k < E; k++) dg[k] = db[k] = 0.f;
   uint32_t turn = 0;
-  for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += gridDim.x * PER_BLOCK, turn ^= 1u) {
+  // the next row is loaded before the row in hand is summed and stored, where the registers allow (1024 threads have 128 each; single
+  // values need an address each).  The error may be written over delta: a row is stored after its own loads, and by the threads that
+  // loaded it
+  constexpr bool EARLY = VEC && L < 1024;
+  const uint32_t stride = gridDim.x * PER_BLOCK;
+  float x[E], g[E], xn[EARLY ? E : 1], gn[EARLY ? E : 1], mean, ivar;
+  const auto load = [&](uint32_t row, float *xr, float (&gr)[E], float *m, float *v) {
+    *m = a.mean[row];
+    *v = a.ivar[row];
+    const auto in = rows.row(row);
+    S::load(gr, a.delta + (size_t)row * a.N, a.N, 0.f);
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(xr + j * W, min(S::first(j), a.N - W));
+  };
+  if constexpr (EARLY) load(min(blockIdx.x * PER_BLOCK + sub, a.rows - 1), x, g, &mean, &ivar);
+  for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += stride, turn ^= 1u) {
     const uint32_t row = min(first + sub, a.rows - 1);
     const bool mine = first + sub < a.rows;
-    const float mean = a.mean[row], ivar = a.ivar[row];
-    const auto in = rows.row(row);
-    float x[E], g[E];
-    S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
-#pragma unroll
-    for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, min(S::first(j), a.N - W));
+    float mean_n, ivar_n;
+    if constexpr (EARLY)
+      load(min(first + stride + sub, a.rows - 1), xn, gn, &mean_n, &ivar_n);
+    else
+      load(row, x, g, &mean, &ivar);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < S::STEPS; j++) {
@@ -379,8 +397,16 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
         S::store(error, j, t);
       }
     }
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int k = 0; k < E; k++) {
+        x[k] = xn[k];
+        g[k] = gn[k];
+      }
+      mean = mean_n;
+      ivar = ivar_n;
+    }
   }
-  if (a.dgamma == nullptr && a.dbeta == nullptr) return;
   float *pg = partial + (size_t)blockIdx.x * a.N, *pb = partial + ((size_t)gridDim.x + blockIdx.x) * a.N;
   if (L >= 256) {
 #pragma unroll
@@ -411,6 +437,87 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     pb[i] = sb;
   }
   (void)lane;
+}
+
+// The error alone, one row per L threads, and beside it in the same launch (blocks from error_blocks on) dgamma and dbeta straight
+// from delta and x: they need no sum over a row.  That reads both a second time, from the caches, where the kernel above writes and
+// joins partial sums: 256 rows of 4096 10.7 -> 5.2 us, 33 of 1001 7.0 -> 4.9; 8192 of 2048 would lose (36 us against 50).
+template <int L, int E, bool VEC, class Rows>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t error_blocks) {
+  using S = Share<L, E, VEC>;
+  constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
+  constexpr int W = S::WIDTH;
+  if (blockIdx.x >= error_blocks) {
+    // BLOCK / 16 columns, sixteen rows at a time with four loads of each operand in flight
+    constexpr uint32_t COLUMNS = BLOCK / 16;
+    __shared__ float sums[2][16][COLUMNS];
+    const uint32_t c = threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS, column = (blockIdx.x - error_blocks) * COLUMNS + c, i = min(column, a.N - 1);
+    float gamma, sg = 0.f, sb = 0.f;
+    load_step<false>(&gamma, a.gamma, i);
+    for (uint32_t k = slice; k < a.rows; k += 64) {
+      float x[4], g[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const uint32_t row = min(k + 16 * u, a.rows - 1);
+        g[u] = a.delta[(size_t)row * a.N + i];
+        rows.row(row).template step<false>(x + u, i);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const uint32_t row = min(k + 16 * u, a.rows - 1);
+        step_terms<1>(a, a.mean[row], a.ivar[row], &gamma, i, x + u, g + u);
+        if (k + 16 * u < a.rows) {
+          sg += g[u] * x[u];
+          sb += g[u];
+        }
+      }
+    }
+    sums[0][slice][c] = sg;
+    sums[1][slice][c] = sb;
+    __syncthreads();
+    if (slice > 1 || column >= a.N) return;
+    float *out = slice == 0 ? a.dgamma : a.dbeta;
+    if (out == nullptr) return;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) s += (sums[slice][k][c] + sums[slice][k + 1][c]) + (sums[slice][k + 2][c] + sums[slice][k + 3][c]);
+    out[column] = a.accumulate ? out[column] + s : s;
+    return;
+  }
+  __shared__ float part[2][L / 64 + 1];
+  const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
+  const float mean = a.mean[row], ivar = a.ivar[row];
+  const auto in = rows.row(row);
+  float x[E], g[E];
+  S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, min(S::first(j), a.N - W));
+  float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) {
+    const uint32_t i = min(S::first(j), a.N - W);
+    float gamma[W];
+    load_step<VEC>(gamma, a.gamma, i);
+    step_terms<W>(a, mean, ivar, gamma, i, x + j * W, g + j * W);
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      const int k = j * W + e;
+      g[k] *= gamma[e];
+      s1 += S::first(j) < a.N ? g[k] : 0.f;
+      s2 += S::first(j) < a.N ? g[k] * x[k] : 0.f;
+    }
+  }
+  s1 = row_sum<L>(s1, part[0]) / (float)a.N;
+  s2 = row_sum<L>(s2, part[1]) / (float)a.N;
+  if (want >= a.rows) return;
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) {
+    if (S::first(j) >= a.N) continue;
+    float t[W];
+#pragma unroll
+    for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
+    S::store(a.error + (size_t)row * a.N, j, t);
+  }
 }
 
 // longer rows: the two sums of every piece ...
@@ -622,6 +729,8 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
   }
   const bool params = dgamma || dbeta;
   const bool vec = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
+  // few rows: the parameter gradients beside the error instead of partial sums and their join
+  const bool few = g.rows <= 512;
   uint32_t parts = 0;
   float *partial = nullptr;
   if (g.N <= BACKWARD_ROW) {
@@ -629,12 +738,29 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
       constexpr int L = l, E = e;
       if constexpr (L * E <= (int)BACKWARD_ROW) {
         const uint32_t per_block = L < 256 ? 256 / L : 1, threads = L < 256 ? 256 : L;
-        parts = cdiv(g.rows, per_block);
-        if (parts > 512) parts = 512;
-        if (params) {
-          int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
-          if (rc) return rc;
+        if (!params || few) {
+          const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
+          const auto go = [&](uint32_t grid, uint32_t first_param_block) {
+            if (vec)
+              ln_backward_few_kernel<L, E, true, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
+            else
+              ln_backward_few_kernel<L, E, false, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
+          };
+          if (a.error == a.delta && params) {  // written in place: the sums before the error
+            go(param_blocks, 0);
+            go(error_blocks, error_blocks);
+          } else {
+            go(error_blocks + param_blocks, error_blocks);
+          }
+          return (int)MT_OK;
         }
+        parts = cdiv(g.rows, per_block);
+        // one block per compute unit: its next row is on the way while it sums, and more blocks mean more partial sums (8192 x 2048: 34.3 us
+        // with 256, 34.9 with 512, 38.3 with 1024; 1024 x 8192: 23.0, 30.6, 41.7); short rows need the second block (60000 x 256: 36.5, 32.8)
+        const uint32_t most = L * E <= 256 ? 512 : 256;
+        if (parts > most) parts = most;
+        int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
+        if (rc) return rc;
         if (vec)
           ln_backward_kernel<L, E, true, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
         else
@@ -646,10 +772,10 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     MT_LAUNCH_CHECK(name);
   } else {
     const uint32_t pieces = cdiv(g.N, PIECE), strips = cdiv(g.N, THREADS * (vec ? 4 : 1));
-    // blocks that walk over all rows (at most 64) where the strips alone are three for four compute units: no partial sums to
-    // write and join.  Shorter rows: groups of at least 16 rows, so that the partial sums stay a twentieth of the traffic
-    uint32_t groups = strips >= 192 ? 1 : cdiv(1024, strips);
-    if (groups > cdiv(g.rows, 16)) groups = cdiv(g.rows, 16);
+    // enough blocks to keep the memory busy, but groups of at least 8 rows: every group writes and joins 16 bytes per column where a
+    // row moves 20
+    uint32_t groups = cdiv(1024, strips);
+    if (groups > cdiv(g.rows, 8)) groups = cdiv(g.rows, 8);
     uint32_t per_group = cdiv(g.rows, groups);
     if (per_group > GROUP_ROWS) per_group = GROUP_ROWS;
     groups = cdiv(g.rows, per_group);
@@ -673,7 +799,10 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     MT_LAUNCH_CHECK(name);
   }
   if (params && parts) {
-    ln_join_kernel<<<dim3(cdiv(g.N, 64), 2), 64 * JOIN_SLICES, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
+    if (parts > JOIN_MANY)
+      ln_join_kernel<JOIN_MANY><<<dim3(cdiv(g.N, 64), 2), 64 * JOIN_MANY, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
+    else
+      ln_join_kernel<1><<<dim3(cdiv(g.N, THREADS), 2), THREADS, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
     MT_LAUNCH_CHECK(name);
   }
   return MT_OK;

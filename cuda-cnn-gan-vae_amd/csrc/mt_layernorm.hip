@@ -34,6 +34,30 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
   return v;
 }
 
+// ---- the functions of the function layer that the kernels hold: the values of f_sigmoid_fast and f_tangence_fast, with a reciprocal
+// that is not a division (two thirds of the instructions; 32 rows of 147456 with sigmoid 12.8 -> 11.8 us) ---------------------------
+__device__ __forceinline__ float sigmoid(float v) {
+  if (v > 30.f) v = 29.99999f;
+  if (v < -30.f) v = -29.99999f;
+  return mt::reciprocal(1.f + __expf(-v));
+}
+__device__ __forceinline__ float tangence(float v) {
+  if (v > 30.f) v = 30.f;  // 1 from there on; an infinite exponential has no reciprocal here
+  return 1.f - 2.f * mt::reciprocal(__expf(2.f * v) + 1.f);
+}
+template <int N>
+__device__ __forceinline__ void apply(int func, float *v) {
+  if (func == MT_F_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = sigmoid(v[i]);
+  } else if (func == MT_F_TANGENCE) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = tangence(v[i]);
+  } else {
+    mt::apply_func_cheap_many<N>(func, v);
+  }
+}
+
 // ---- how the L threads of a row share its N values: E each, in vectors of four 4 * L apart, or singly L apart ----------------
 template <int L, int E, bool VEC>
 struct Share {
@@ -147,7 +171,7 @@ __device__ __forceinline__ void normalise(const Forward &a, float *out, const fl
     load_step<VEC>(b, beta, S::first(j));
 #pragma unroll
     for (int e = 0; e < S::WIDTH; e++) y[e] = g[e] * ((x[j * S::WIDTH + e] - mean) * ivar) + b[e];
-    mt::apply_func_epilogue_many<S::WIDTH>(a.func, y);
+    apply<S::WIDTH>(a.func, y);
     S::store(out, j, y);
   }
 }
@@ -255,28 +279,28 @@ struct Backward {
   bool accumulate;
 };
 
-// delta * f'(gamma * xhat + beta) for the functions that the kernels hold inline
-__device__ __forceinline__ float front(int func, float delta, float gamma, float xhat, float beta) {
-  const float pre = gamma * xhat + beta;
-  if (func == MT_F_RELU) return pre >= 0.f ? delta : delta * 0.f;
-  if (func == MT_F_LEAKY_RELU) return delta * (pre >= 0.f ? 1.f : 0.1f);
-  if (func == MT_F_SIGMOID) {
-    const float f = mt::f_sigmoid_fast(pre);
-    return delta * ((1.f - f) * f);
-  }
-  const float f = mt::f_tangence_fast(pre);
-  return delta * (1.f - f * f);
-}
-// xhat and the gradient in front of the function for one step of a row
-template <int WIDTH>
-__device__ __forceinline__ void step_terms(const Backward &a, float mean, float ivar, const float *gamma, uint32_t at, float *x, float *g) {
+// delta * f'(gamma * xhat + beta) for N values, one look at the (uniform) function for all of them; the kernels are compiled with and
+// without a function (a look per value and a load of beta at every step made 8192 x 2048 take 81 us with tangence, 34 without)
+template <int N>
+__device__ __forceinline__ void fronts(int func, float *g, const float *gamma, const float *xhat, const float *beta) {
+  if (func == MT_F_RELU) {
 #pragma unroll
-  for (int e = 0; e < WIDTH; e++) x[e] = (x[e] - mean) * ivar;
-  if (a.func != MT_F_NONE) {
-    float b[WIDTH];
-    load_step<WIDTH == 4>(b, a.beta, at);
+    for (int i = 0; i < N; i++) g[i] *= gamma[i] * xhat[i] + beta[i] >= 0.f ? 1.f : 0.f;
+  } else if (func == MT_F_LEAKY_RELU) {
 #pragma unroll
-    for (int e = 0; e < WIDTH; e++) g[e] = front(a.func, g[e], gamma[e], x[e], b[e]);
+    for (int i = 0; i < N; i++) g[i] *= gamma[i] * xhat[i] + beta[i] >= 0.f ? 1.f : 0.1f;
+  } else if (func == MT_F_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float f = sigmoid(gamma[i] * xhat[i] + beta[i]);
+      g[i] *= (1.f - f) * f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float f = tangence(gamma[i] * xhat[i] + beta[i]);
+      g[i] *= 1.f - f * f;
+    }
   }
 }
 
@@ -314,7 +338,7 @@ __global__ __launch_bounds__(SLICES == 1 ? THREADS : 64 * SLICES) void ln_join_k
 }
 
 // rows that fit the registers of L threads; a block walks over the rows and keeps its share of dgamma and dbeta in registers
-template <int L, int E, bool VEC, class Rows>
+template <int L, int E, bool VEC, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
@@ -322,8 +346,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
   __shared__ float part[2][2][L / 64 + 1];
   __shared__ float shared[L < 256 ? 2 * 256 * E : 1];
   const uint32_t sub = threadIdx.x / L, lane = threadIdx.x % L;
-  float dg[E], db[E], gamma[E];
+  float dg[E], db[E], gamma[E], beta[FUNC ? E : 1];
   S::load(gamma, a.gamma, a.N, 0.f);
+  if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
 #pragma unroll
   for (int k = 0; k < E; k++) dg[k] = db[k] = 0.f;
   uint32_t turn = 0;
@@ -352,8 +377,10 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
       load(row, x, g, &mean, &ivar);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
+    for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
+    if constexpr (FUNC) fronts<E>(a.func, g, gamma, x, beta);
+#pragma unroll
     for (int j = 0; j < S::STEPS; j++) {
-      step_terms<W>(a, mean, ivar, gamma + j * W, min(S::first(j), a.N - W), x + j * W, g + j * W);
 #pragma unroll
       for (int e = 0; e < W; e++) {
         const int k = j * W + e;
@@ -442,7 +469,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 // The error alone, one row per L threads, and beside it in the same launch (blocks from error_blocks on) dgamma and dbeta straight
 // from delta and x: they need no sum over a row.  That reads both a second time, from the caches, where the kernel above writes and
 // joins partial sums: 256 rows of 4096 10.7 -> 5.2 us, 33 of 1001 7.0 -> 4.9; 8192 of 2048 would lose (36 us against 50).
-template <int L, int E, bool VEC, class Rows>
+template <int L, int E, bool VEC, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t error_blocks) {
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
@@ -452,8 +479,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
     constexpr uint32_t COLUMNS = BLOCK / 16;
     __shared__ float sums[2][16][COLUMNS];
     const uint32_t c = threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS, column = (blockIdx.x - error_blocks) * COLUMNS + c, i = min(column, a.N - 1);
-    float gamma, sg = 0.f, sb = 0.f;
-    load_step<false>(&gamma, a.gamma, i);
+    float gamma[4], beta[4] = {}, sg = 0.f, sb = 0.f;
+    gamma[0] = gamma[1] = gamma[2] = gamma[3] = a.gamma[i];
+    if (FUNC) beta[0] = beta[1] = beta[2] = beta[3] = a.beta[i];
     for (uint32_t k = slice; k < a.rows; k += 64) {
       float x[4], g[4];
 #pragma unroll
@@ -461,11 +489,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
         const uint32_t row = min(k + 16 * u, a.rows - 1);
         g[u] = a.delta[(size_t)row * a.N + i];
         rows.row(row).template step<false>(x + u, i);
+        x[u] = (x[u] - a.mean[row]) * a.ivar[row];
       }
+      if constexpr (FUNC) fronts<4>(a.func, g, gamma, x, beta);
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const uint32_t row = min(k + 16 * u, a.rows - 1);
-        step_terms<1>(a, a.mean[row], a.ivar[row], &gamma, i, x + u, g + u);
         if (k + 16 * u < a.rows) {
           sg += g[u] * x[u];
           sb += g[u];
@@ -492,17 +520,19 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
   S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, min(S::first(j), a.N - W));
+  float gamma[E], beta[FUNC ? E : 1];
+  S::load(gamma, a.gamma, a.N, 0.f);
+  if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
+  for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
+  if constexpr (FUNC) fronts<E>(a.func, g, gamma, x, beta);
+#pragma unroll
   for (int j = 0; j < S::STEPS; j++) {
-    const uint32_t i = min(S::first(j), a.N - W);
-    float gamma[W];
-    load_step<VEC>(gamma, a.gamma, i);
-    step_terms<W>(a, mean, ivar, gamma, i, x + j * W, g + j * W);
 #pragma unroll
     for (int e = 0; e < W; e++) {
       const int k = j * W + e;
-      g[k] *= gamma[e];
+      g[k] *= gamma[k];
       s1 += S::first(j) < a.N ? g[k] : 0.f;
       s2 += S::first(j) < a.N ? g[k] * x[k] : 0.f;
     }
@@ -521,7 +551,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
 }
 
 // longer rows: the two sums of every piece ...
-template <bool VEC, class Rows>
+template <bool VEC, bool FUNC, class Rows>
 __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a, Rows rows, float2 *sums, uint32_t pieces) {
   using S = Share<THREADS, PIECE / THREADS, VEC>;
   constexpr int W = S::WIDTH;
@@ -533,16 +563,18 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
   S::load(g, a.delta + (size_t)row * a.N + at, n, 0.f);
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, at + min(S::first(j), n - W));
+  float gamma[PIECE / THREADS], beta[FUNC ? PIECE / THREADS : 1];
+  S::load(gamma, a.gamma + at, n, 0.f);
+  if constexpr (FUNC) S::load(beta, a.beta + at, n, 0.f);
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
+  for (int k = 0; k < (int)(PIECE / THREADS); k++) x[k] = (x[k] - mean) * ivar;
+  if constexpr (FUNC) fronts<PIECE / THREADS>(a.func, g, gamma, x, beta);
+#pragma unroll
   for (int j = 0; j < S::STEPS; j++) {
-    const uint32_t i = at + min(S::first(j), n - W);
-    float gamma[W];
-    load_step<VEC>(gamma, a.gamma, i);
-    step_terms<W>(a, mean, ivar, gamma, i, x + j * W, g + j * W);
 #pragma unroll
     for (int e = 0; e < W; e++) {
-      const float u = S::first(j) < n ? g[j * W + e] * gamma[e] : 0.f;
+      const float u = S::first(j) < n ? g[j * W + e] * gamma[j * W + e] : 0.f;
       s1 += u;
       s2 += S::first(j) < n ? u * x[j * W + e] : 0.f;
     }
@@ -553,7 +585,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
 }
 // ... then blocks of 256 * WIDTH columns that walk over a group of rows: the error, and their columns' share of dgamma and dbeta
 constexpr uint32_t GROUP_ROWS = 64;  // rows of a group, at most
-template <bool VEC, class Rows>
+template <bool VEC, bool FUNC, class Rows>
 __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a, Rows rows, const float2 *sums, uint32_t pieces, uint32_t groups, uint32_t per_group,
                                                                      float *partial) {
   constexpr int W = VEC ? 4 : 1;
@@ -571,12 +603,17 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
     s2 = mt::over_lanes<mt::Sum, 64>(s2) / (float)a.N;
     if (lane == 0) terms[k] = make_float4(a.mean[first + k], a.ivar[first + k], s1, s2);
   }
-  float gamma[W], dg[W] = {}, db[W] = {};
-  load_step<VEC>(gamma, a.gamma, at);
+  // gamma and beta repeated for the rows that are taken at once
+  constexpr uint32_t AT_ONCE = 4;
+  float gamma[AT_ONCE][W], beta[AT_ONCE][W], dg[W] = {}, db[W] = {};
+#pragma unroll
+  for (uint32_t u = 0; u < AT_ONCE; u++) {
+    load_step<VEC>(gamma[u], a.gamma, at);
+    if (FUNC) load_step<VEC>(beta[u], a.beta, at);
+  }
   __syncthreads();
   // four rows at a time, loaded before the first of them is stored (the error may be written over delta: each thread reads and
   // writes its own columns)
-  constexpr uint32_t AT_ONCE = 4;
   for (uint32_t k0 = 0; k0 < count; k0 += AT_ONCE) {
     float x[AT_ONCE][W], g[AT_ONCE][W];
 #pragma unroll
@@ -587,15 +624,21 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
     }
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
+      const float4 c = terms[min(k0 + u, count - 1)];
+#pragma unroll
+      for (int e = 0; e < W; e++) x[u][e] = (x[u][e] - c.x) * c.y;
+    }
+    if constexpr (FUNC) fronts<AT_ONCE * W>(a.func, g[0], gamma[0], x[0], beta[0]);
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; u++) {
       if (k0 + u >= count) break;
       const float4 c = terms[k0 + u];
       float t[W];
-      step_terms<W>(a, c.x, c.y, gamma, at, x[u], g[u]);
 #pragma unroll
       for (int e = 0; e < W; e++) {
         dg[e] += g[u][e] * x[u][e];
         db[e] += g[u][e];
-        t[e] = c.y * ((g[u][e] * gamma[e] - c.z) - x[u][e] * c.w);
+        t[e] = c.y * ((g[u][e] * gamma[u][e] - c.z) - x[u][e] * c.w);
       }
       if (column < a.N) {
         float *p = a.error + (size_t)(first + k0 + u) * a.N + column;
@@ -713,6 +756,16 @@ int with_share(uint32_t N, F &&f) {
   return f(integral_constant<int, 1024>{}, integral_constant<int, 32>{});
 }
 
+// calls f with what a kernel is compiled for
+template <class F>
+void with_kind(bool vec, bool func, F &&f) {
+  if (vec) {
+    if (func) f(std::true_type{}, std::true_type{}); else f(std::true_type{}, std::false_type{});
+  } else {
+    if (func) f(std::false_type{}, std::true_type{}); else f(std::false_type{}, std::false_type{});
+  }
+}
+
 template <class Rows>
 int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, const mt_tensor *dbeta, const mt_tensor *delta, const mt_tensor *gamma,
              const mt_tensor *beta, const Rows &x, bool x_aligned, const mt_tensor *mean, const mt_tensor *ivar, int func, int accumulate, const Geometry &g) {
@@ -741,10 +794,9 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         if (!params || few) {
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
           const auto go = [&](uint32_t grid, uint32_t first_param_block) {
-            if (vec)
-              ln_backward_few_kernel<L, E, true, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
-            else
-              ln_backward_few_kernel<L, E, false, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
+            with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
+              ln_backward_few_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
+            });
           };
           if (a.error == a.delta && params) {  // written in place: the sums before the error
             go(param_blocks, 0);
@@ -761,10 +813,9 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         if (parts > most) parts = most;
         int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
         if (rc) return rc;
-        if (vec)
-          ln_backward_kernel<L, E, true, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
-        else
-          ln_backward_kernel<L, E, false, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+        with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
+          ln_backward_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+        });
       }
       return (int)MT_OK;
     });
@@ -787,15 +838,11 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     float2 *piece_sums = reinterpret_cast<float2 *>(ws);
     partial = ws + sums;
     parts = groups > 1 ? groups : 0;
-    if (vec) {
-      ln_backward_pieces_kernel<true><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
-      MT_LAUNCH_CHECK(name);
-      ln_backward_columns_kernel<true><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
-    } else {
-      ln_backward_pieces_kernel<false><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
-      MT_LAUNCH_CHECK(name);
-      ln_backward_columns_kernel<false><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
-    }
+    with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
+      constexpr bool VEC = decltype(v)::value, FUNC = decltype(f)::value;
+      ln_backward_pieces_kernel<VEC, FUNC><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
+      ln_backward_columns_kernel<VEC, FUNC><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
+    });
     MT_LAUNCH_CHECK(name);
   }
   if (params && parts) {

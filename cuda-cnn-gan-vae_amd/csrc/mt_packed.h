@@ -63,6 +63,13 @@ inline bool overlap(const mt_tensor *a, const mt_tensor *b) { return overlap(a->
 inline bool overlap(const mt_tensor *a, const PackedView &b) { return overlap(a->p, count(a) * 4, b.q, packed_bytes(b)); }
 
 // ---- device side ---------------------------------------------------------------------------------------------------
+// 1 / y for a normal y up to 2^125, correctly rounded: the hardware's reciprocal and one step of Newton's method give the rounded
+// quotient for every mantissa (all 2^23 compared with the division at ten exponents), without the ten instructions of a division
+__device__ __forceinline__ float reciprocal(float y) {
+  const float r = __builtin_amdgcn_rcpf(y);
+  return __builtin_fmaf(__builtin_fmaf(-y, r, 1.f), r, r);
+}
+
 // (low, step, 1/step) of a group from its lowest and highest value.  A range that is not a finite number (a NaN or an
 // infinity in the group, or values 3.4e38 apart) makes every value of the group NaN: what was lost shows.  A step below the
 // smallest normal number counts as none, so that its reciprocal exists.
@@ -76,11 +83,7 @@ __device__ __forceinline__ PackScale pack_scale(float low, float high) {
   s.step = finite ? range * (1.f / 255.f) : 0.f;
   if (s.step < FLT_MIN) s.step = 0.f;
   s.low = finite ? low : __int_as_float(0x7fc00000);
-  // 1 / step, correctly rounded: the hardware's reciprocal and one step of Newton's method give the rounded quotient for every
-  // mantissa (all 2^23 compared with the division at ten exponents), without the scaling that a division does for
-  // subnormal numbers
-  const float r = __builtin_amdgcn_rcpf(s.step);
-  s.inverse = s.step > 0.f ? __builtin_fmaf(__builtin_fmaf(-s.step, r, 1.f), r, r) : 0.f;
+  s.inverse = s.step > 0.f ? reciprocal(s.step) : 0.f;
   return s;
 }
 // the count of steps put into byte k of w: the instruction rounds half to even and holds the result within 0..255

@@ -97,35 +97,47 @@ __device__ __forceinline__ void load_step(float *t, const float *p, uint32_t at)
   }
 }
 
-// ---- where a row's input comes from in the backward pass: the fp32 tensor, or the 8 bits the forward pass kept ------------
+// ---- where a row's input comes from in the backward pass: the fp32 tensor, or the 8 bits the forward pass kept.  Loading and
+// decoding are two steps, so that all loads of a row are under way before the first is waited for ------------------------------
 struct RowsF32 {
   const float *p;
   uint32_t N;
+  template <bool VEC>
+  struct Raw {
+    float t[VEC ? 4 : 1];
+    __device__ __forceinline__ void values(float *x) const {
+#pragma unroll
+      for (int k = 0; k < (VEC ? 4 : 1); k++) x[k] = t[k];
+    }
+  };
   struct Row {
     const float *p;
     template <bool VEC>
-    __device__ __forceinline__ void step(float *t, uint32_t at) const { load_step<VEC>(t, p, at); }
+    __device__ __forceinline__ void load(Raw<VEC> &raw, uint32_t at) const { load_step<VEC>(raw.t, p, at); }
   };
   __device__ __forceinline__ Row row(uint32_t r) const { return Row{p + (size_t)r * N}; }
 };
 struct RowsPacked {
   PackedView v;
   uint32_t N, per_sample;  // rows of one sample
+  template <bool VEC>
+  struct Raw {
+    float2 pair;
+    uint32_t q;
+    __device__ __forceinline__ void values(float *x) const {
+#pragma unroll
+      for (int k = 0; k < (VEC ? 4 : 1); k++) x[k] = mt::unpack_value(pair, VEC ? (q >> (8 * k)) & 255u : q);
+    }
+  };
   struct Row {
     const uint8_t *q;
     const float2 *pair;
     uint32_t first;  // the row's first value within its sample
     template <bool VEC>
-    __device__ __forceinline__ void step(float *t, uint32_t at) const {
+    __device__ __forceinline__ void load(Raw<VEC> &raw, uint32_t at) const {
       const uint32_t e = first + at;
-      const float2 s = pair[e / mt::PACK_GROUP];
-      if (VEC) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(q + e);
-#pragma unroll
-        for (int k = 0; k < 4; k++) t[k] = mt::unpack_value(s, (w >> (8 * k)) & 255u);
-      } else {
-        t[0] = mt::unpack_value(s, q[e]);
-      }
+      raw.pair = pair[e / mt::PACK_GROUP];
+      raw.q = VEC ? *reinterpret_cast<const uint32_t *>(q + e) : q[e];
     }
   };
   __device__ __forceinline__ Row row(uint32_t r) const {
@@ -346,9 +358,13 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
   __shared__ float part[2][2][L / 64 + 1];
   __shared__ float shared[L < 256 ? 2 * 256 * E : 1];
   const uint32_t sub = threadIdx.x / L, lane = threadIdx.x % L;
+  constexpr bool HELD = L < 1024;  // gamma and beta stay in registers; 1024 threads load them for every row
   float dg[E], db[E], gamma[E], beta[FUNC ? E : 1];
-  S::load(gamma, a.gamma, a.N, 0.f);
-  if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
+  const auto load_parameters = [&] {
+    S::load(gamma, a.gamma, a.N, 0.f);
+    if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
+  };
+  if constexpr (HELD) load_parameters();
 #pragma unroll
   for (int k = 0; k < E; k++) dg[k] = db[k] = 0.f;
   uint32_t turn = 0;
@@ -357,24 +373,30 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
   // loaded it
   constexpr bool EARLY = VEC && L < 1024;
   const uint32_t stride = gridDim.x * PER_BLOCK;
-  float x[E], g[E], xn[EARLY ? E : 1], gn[EARLY ? E : 1], mean, ivar;
-  const auto load = [&](uint32_t row, float *xr, float (&gr)[E], float *m, float *v) {
+  typedef typename Rows::template Raw<VEC> Raw;
+  Raw raw[S::STEPS], next[EARLY ? S::STEPS : 1];
+  float x[E], g[E], gn[EARLY ? E : 1], mean, ivar;
+  const auto load = [&](uint32_t row, Raw *r, float (&gr)[E], float *m, float *v) {
     *m = a.mean[row];
     *v = a.ivar[row];
     const auto in = rows.row(row);
     S::load(gr, a.delta + (size_t)row * a.N, a.N, 0.f);
 #pragma unroll
-    for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(xr + j * W, min(S::first(j), a.N - W));
+    for (int j = 0; j < S::STEPS; j++) in.load(r[j], min(S::first(j), a.N - W));
   };
-  if constexpr (EARLY) load(min(blockIdx.x * PER_BLOCK + sub, a.rows - 1), x, g, &mean, &ivar);
+  if constexpr (EARLY) load(min(blockIdx.x * PER_BLOCK + sub, a.rows - 1), raw, g, &mean, &ivar);
   for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += stride, turn ^= 1u) {
     const uint32_t row = min(first + sub, a.rows - 1);
     const bool mine = first + sub < a.rows;
     float mean_n, ivar_n;
     if constexpr (EARLY)
-      load(min(first + stride + sub, a.rows - 1), xn, gn, &mean_n, &ivar_n);
+      load(min(first + stride + sub, a.rows - 1), next, gn, &mean_n, &ivar_n);
     else
-      load(row, x, g, &mean, &ivar);
+      load(row, raw, g, &mean, &ivar);
+    if constexpr (!HELD) load_parameters();
+    __builtin_amdgcn_sched_barrier(0);  // all loads before the first use of one
+#pragma unroll
+    for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
@@ -426,10 +448,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     }
     if constexpr (EARLY) {
 #pragma unroll
-      for (int k = 0; k < E; k++) {
-        x[k] = xn[k];
-        g[k] = gn[k];
-      }
+      for (int j = 0; j < S::STEPS; j++) raw[j] = next[j];
+#pragma unroll
+      for (int k = 0; k < E; k++) g[k] = gn[k];
       mean = mean_n;
       ivar = ivar_n;
     }
@@ -483,13 +504,21 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
     gamma[0] = gamma[1] = gamma[2] = gamma[3] = a.gamma[i];
     if (FUNC) beta[0] = beta[1] = beta[2] = beta[3] = a.beta[i];
     for (uint32_t k = slice; k < a.rows; k += 64) {
-      float x[4], g[4];
+      typename Rows::template Raw<false> raw[4];
+      float x[4], g[4], mean[4], ivar[4];
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const uint32_t row = min(k + 16 * u, a.rows - 1);
         g[u] = a.delta[(size_t)row * a.N + i];
-        rows.row(row).template step<false>(x + u, i);
-        x[u] = (x[u] - a.mean[row]) * a.ivar[row];
+        rows.row(row).load(raw[u], i);
+        mean[u] = a.mean[row];
+        ivar[u] = a.ivar[row];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        raw[u].values(x + u);
+        x[u] = (x[u] - mean[u]) * ivar[u];
       }
       if constexpr (FUNC) fronts<4>(a.func, g, gamma, x, beta);
 #pragma unroll
@@ -516,13 +545,16 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
   const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
   const float mean = a.mean[row], ivar = a.ivar[row];
   const auto in = rows.row(row);
-  float x[E], g[E];
+  typename Rows::template Raw<VEC> raw[S::STEPS];
+  float x[E], g[E], gamma[E], beta[FUNC ? E : 1];
   S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, min(S::first(j), a.N - W));
-  float gamma[E], beta[FUNC ? E : 1];
+  for (int j = 0; j < S::STEPS; j++) in.load(raw[j], min(S::first(j), a.N - W));
   S::load(gamma, a.gamma, a.N, 0.f);
   if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
@@ -559,13 +591,17 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE), at = piece * PIECE;
   const float mean = a.mean[row], ivar = a.ivar[row];
   const auto in = rows.row(row);
+  typename Rows::template Raw<VEC> raw[S::STEPS];
   float x[PIECE / THREADS], g[PIECE / THREADS];
   S::load(g, a.delta + (size_t)row * a.N + at, n, 0.f);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.template step<VEC>(x + j * W, at + min(S::first(j), n - W));
+  for (int j = 0; j < S::STEPS; j++) in.load(raw[j], at + min(S::first(j), n - W));
   float gamma[PIECE / THREADS], beta[FUNC ? PIECE / THREADS : 1];
   S::load(gamma, a.gamma + at, n, 0.f);
   if constexpr (FUNC) S::load(beta, a.beta + at, n, 0.f);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int k = 0; k < (int)(PIECE / THREADS); k++) x[k] = (x[k] - mean) * ivar;
@@ -615,15 +651,18 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
   // four rows at a time, loaded before the first of them is stored (the error may be written over delta: each thread reads and
   // writes its own columns)
   for (uint32_t k0 = 0; k0 < count; k0 += AT_ONCE) {
+    typename Rows::template Raw<VEC> raw[AT_ONCE];
     float x[AT_ONCE][W], g[AT_ONCE][W];
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
       const uint32_t row = first + min(k0 + u, count - 1);
       load_step<VEC>(g[u], a.delta + (size_t)row * a.N, at);
-      rows.row(row).template step<VEC>(x[u], at);
+      rows.row(row).load(raw[u], at);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
+      raw[u].values(x[u]);
       const float4 c = terms[min(k0 + u, count - 1)];
 #pragma unroll
       for (int e = 0; e < W; e++) x[u][e] = (x[u][e] - c.x) * c.y;
@@ -675,8 +714,10 @@ __global__ __launch_bounds__(THREADS) void ln_front_kernel(Backward a, Rows rows
     const float mean = a.mean[row], ivar = a.ivar[row];
     const auto in = rows.row(row);
     for (uint32_t i = blockIdx.y * THREADS + threadIdx.x; i < a.N; i += gridDim.y * THREADS) {
+      typename Rows::template Raw<false> raw;
       float x;
-      in.template step<false>(&x, i);
+      in.load(raw, i);
+      raw.values(&x);
       const size_t e = (size_t)row * a.N + i;
       a.error[e] = a.delta[e] * mt::apply_func(MT_F_DIFFERENTIAL + a.func, a.gamma[i] * ((x - mean) * ivar) + a.beta[i]);
     }
@@ -719,8 +760,10 @@ int geometry(const char *name, const mt_tensor *in, const mt_tensor *gamma, Geom
 bool same_sizes(const mt_tensor *a, const mt_tensor *b) { return mt::same_zyx(a, b) && a->w == b->w; }
 bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { return t->w == in->w && t->z == g.kept_z && t->y == g.kept_y && t->x == 1; }
 
-// rows of up to this many values are held in registers
-constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384;
+// rows of up to this many values are held in registers.  In the backward pass 1024 threads have room for 16 values each and their
+// share of two sums, but not for a function's parameters or an address per value too: 2000 x 16384 with tangence 134 us against 114 in
+// pieces, 2000 x 16383 185 against 129
+constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384, BACKWARD_ROW_TIGHT = 8192;
 
 template <int L, int E>
 void forward_rows(const Forward &a, bool vec, bool pack) {
@@ -786,12 +829,13 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
   const bool few = g.rows <= 512;
   uint32_t parts = 0;
   float *partial = nullptr;
-  if (g.N <= BACKWARD_ROW) {
+  const bool beside = !params || few;  // no sums over rows in the error's threads
+  if (g.N <= (beside || (vec && a.func == MT_F_NONE) ? BACKWARD_ROW : BACKWARD_ROW_TIGHT)) {
     int rc = with_share(g.N, [&](auto l, auto e) {
       constexpr int L = l, E = e;
       if constexpr (L * E <= (int)BACKWARD_ROW) {
         const uint32_t per_block = L < 256 ? 256 / L : 1, threads = L < 256 ? 256 : L;
-        if (!params || few) {
+        if (beside) {
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
           const auto go = [&](uint32_t grid, uint32_t first_param_block) {
             with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
@@ -807,9 +851,10 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
           return (int)MT_OK;
         }
         parts = cdiv(g.rows, per_block);
-        // one block per compute unit: its next row is on the way while it sums, and more blocks mean more partial sums (8192 x 2048: 34.3 us
-        // with 256, 34.9 with 512, 38.3 with 1024; 1024 x 8192: 23.0, 30.6, 41.7); short rows need the second block (60000 x 256: 36.5, 32.8)
-        const uint32_t most = L * E <= 256 ? 512 : 256;
+        // one block per compute unit: its next row is on the way while it sums, and more blocks mean more partial sums (4096 x 6144: 60.0 us
+        // with 256, 66.1 with 512, 74.7 with 1024; 1024 x 8192: 23.0, 30.6, 41.7).  Two where a thread holds few values or loads them
+        // singly and the rows are many (8192 x 2048 from 8 bits 35.4 us with 256, 29.9 with 512; 1024 x 2048 10.7, 12.9)
+        const uint32_t most = (E <= 8 || !vec) && parts >= 4096 ? 512 : 256;
         if (parts > most) parts = most;
         int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
         if (rc) return rc;

@@ -110,9 +110,8 @@ def _row_shape(case):
 
 
 def _bindings():
-    folder = os.path.abspath("cuda-cnn-gan-vae_amd")
-    if folder not in sys.path:
-        sys.path.insert(0, folder)
+    if "mi355tensor" not in sys.modules:
+        sys.path.insert(0, os.path.abspath("cuda-cnn-gan-vae_amd"))
     import mi355tensor
     return mi355tensor
 

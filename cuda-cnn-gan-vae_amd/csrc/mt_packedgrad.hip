@@ -23,7 +23,7 @@ using mt::cdiv;
 using mt::PackedView;
 using mt::xcd_swizzle;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;    // of one group of four wavefronts
 constexpr uint32_t KSTEP = 64;  // samples per step
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -57,13 +57,12 @@ struct WgradSums {
   float offset[TM], bias[TM];    // the second sum and the sum of delta: row lane % 32, half of the samples each
 };
 
-// the product over the samples k0 ... k1.  The sum of delta is taken by all blocks though only those of the first group need it:
+// the product over the samples k0 ... k1 (`steps` steps; those behind k1 add nothing).  The sum of delta is taken by all blocks though only those of the first group need it:
 // one addition in ten, where a second copy of the loop made those blocks the last ones (and the kernel's code twice as long).
 template <int TM>
-__device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g, uint32_t m0, uint32_t k0, uint32_t k1, uintx4 (*cols)[KSTEP / 8][128], float2 (*scale)[KSTEP],
-                                                  WgradSums<TM> &sums) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 31u, half = lane >> 5;
-  const uint32_t steps = (k1 - k0 + KSTEP - 1) / KSTEP;
+__device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g, uint32_t m0, uint32_t k0, uint32_t k1, uint32_t steps, uintx4 (*cols)[KSTEP / 8][128],
+                                                  float2 (*scale)[KSTEP], WgradSums<TM> &sums) {
+  const uint32_t tid = threadIdx.x % THREADS, lane = tid & 63u, r = lane & 31u, half = lane >> 5;
   // this lane's rows r * TM ... of eight samples, AHEAD times 16 samples ahead of the products: 16 where two row tiles fill the
   // registers (two wavefronts per SIMD hide the rest), a whole step where there is room and often one wavefront
   constexpr int AHEAD = TM == 1 ? 4 : 1;
@@ -166,49 +165,16 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
   }
 }
 
-template <int TM>
-__global__ __launch_bounds__(THREADS, 2) void packed_wgrad_kernel(WgradArgs a) {
-  __shared__ uintx4 cols[2][KSTEP / 8][128];  // [eight samples][column]
-  __shared__ float2 scale[2][KSTEP];          // (step, low + 128 * step)
-  __shared__ float4 offsets[4][TM][8];        // the second sum of every row of a wavefront
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, r = lane & 31u, half = lane >> 5;
-  // neighbouring blocks of an XCD share their rows of delta (the larger operand) and walk over the groups
-  uint32_t t = __builtin_amdgcn_readfirstlane(xcd_swizzle(blockIdx.x, gridDim.x));
-  const uint32_t g = t % a.in.groups;
-  t /= a.in.groups;
-  const uint32_t m0 = (t % a.tiles_m) * (128u * TM) + wave * (32u * TM), part = t / a.tiles_m;
-  const uint32_t k0 = part * a.per_split, k1 = min(a.in.w, k0 + a.per_split);
-  const bool bias = a.dbias != nullptr && g == 0;
-  WgradSums<TM> sums;
-#pragma unroll
-  for (int m = 0; m < TM; m++) {
-    sums.offset[m] = sums.bias[m] = 0.f;
-#pragma unroll
-    for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
-  }
-  packed_wgrad_loop<TM>(a, g, m0, k0, k1, cols, scale, sums);
-
-  float *dw = a.dweight, *db = a.dbias;
-  if (a.split > 1) {
-    dw += (size_t)part * a.Out * a.in.n;
-    if (bias) db += (size_t)part * a.Out;
-  }
-#pragma unroll
-  for (int m = 0; m < TM; m++) {
-    const float c = sums.offset[m] + __shfl_xor(sums.offset[m], 32, 64), sum = sums.bias[m] + __shfl_xor(sums.bias[m], 32, 64);
-    if (half == 0) reinterpret_cast<float *>(offsets[wave][m])[r] = c;
-    if (bias && half == 0 && m0 + r * TM + m < a.Out) {
-      float *p = db + m0 + r * TM + m;
-      *p = a.accumulate ? *p + sum : sum;
-    }
-  }
-  __syncthreads();
+// Stores column tiles N0 ... N1 of a wavefront's sums
+template <int TM, int N0, int N1>
+__device__ __forceinline__ void packed_wgrad_store(const WgradArgs &a, float *dw, uint32_t g, uint32_t m0, const float4 (*offsets)[8], const WgradSums<TM> &sums) {
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 31u, half = lane >> 5;
   // accumulator i of tile (m, n): row 8 * (i / 4) + 4 * half + i % 4, column 32 * n + r.  Rows and columns that do not exist have
   // offsets behind the end of the buffer: their stores are dropped
   const uint32_t row_bytes = a.in.n * 4u;
   uint32_t voff[4];
 #pragma unroll
-  for (int n = 0; n < 4; n++) {
+  for (int n = N0; n < N1; n++) {
     const uint32_t c = g * 128u + n * 32u + r;
     voff[n] = c < a.in.n ? 4u * half * TM * row_bytes + c * 4u : 0x80000000u;
   }
@@ -218,37 +184,146 @@ __global__ __launch_bounds__(THREADS, 2) void packed_wgrad_kernel(WgradArgs a) {
     const auto rsrc = rows_rsrc(dw + (size_t)o0 * a.in.n, (int)a.Out - (int)o0, 8 * TM, row_bytes);
 #pragma unroll
     for (int m = 0; m < TM; m++) {
-      const float4 c4 = offsets[wave][m][i4 * 2 + half];
+      const float4 c4 = offsets[m][i4 * 2 + half];
       const float c[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const uint32_t row = (i * TM + m) * row_bytes;
         float v[4];
 #pragma unroll
-        for (int n = 0; n < 4; n++) v[n] = sums.acc[m][n][i4 * 4 + i] + c[i];
+        for (int n = N0; n < N1; n++) v[n] = sums.acc[m][n][i4 * 4 + i] + c[i];
         if (a.accumulate) {
 #pragma unroll
-          for (int n = 0; n < 4; n++) v[n] += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(voff[n] + row), 0, 0));
+          for (int n = N0; n < N1; n++) v[n] += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(voff[n] + row), 0, 0));
         }
 #pragma unroll
-        for (int n = 0; n < 4; n++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[n]), rsrc, (int)(voff[n] + row), 0, 0);
+        for (int n = N0; n < N1; n++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[n]), rsrc, (int)(voff[n] + row), 0, 0);
       }
     }
   }
 }
 
-// the parts of a split sum, added in their order: first the weights' n values, then the bias's Out
+// KW groups of four wavefronts per block.  Two groups take half of the block's samples each, with their own columns in LDS, and add
+// their sums at the end: where the tiles are few, the second wavefront per SIMD that fills the first one's waits comes from the
+// same tile instead of from another part of the batch, whose sums would go through memory.
+template <int TM, int KW>
+__global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(WgradArgs a) {
+  __shared__ uintx4 cols[KW][2][KSTEP / 8][128];  // [eight samples][column]
+  __shared__ float2 scale[KW][2][KSTEP];          // (step, low + 128 * step)
+  __shared__ float4 offsets[4][TM][8];            // the second sum of every row of a wavefront
+  __shared__ float halves[KW > 1 ? 2 : 1][4][TM][32];
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 31u, half = lane >> 5;
+  const uint32_t kw = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u % 4u);
+  // neighbouring blocks of an XCD share their rows of delta (the larger operand) and walk over the groups
+  uint32_t t = __builtin_amdgcn_readfirstlane(xcd_swizzle(blockIdx.x, gridDim.x));
+  const uint32_t g = t % a.in.groups;
+  t /= a.in.groups;
+  const uint32_t m0 = (t % a.tiles_m) * (128u * TM) + wave * (32u * TM), part = t / a.tiles_m;
+  const uint32_t k0 = part * a.per_split, k1 = min(a.in.w, k0 + a.per_split);
+  const uint32_t steps = ((k1 - k0 + KSTEP - 1) / KSTEP + KW - 1) / KW;  // of each group
+  const bool bias = a.dbias != nullptr && g == 0;
+  WgradSums<TM> sums;
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    sums.offset[m] = sums.bias[m] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
+  }
+  const uint32_t first = min(k1, k0 + kw * steps * KSTEP), last = min(k1, first + steps * KSTEP);
+  packed_wgrad_loop<TM>(a, g, m0, first, last, steps, cols[kw], scale[kw], sums);
+
+  float *dw = a.dweight, *db = a.dbias;
+  if (a.split > 1) {
+    dw += (size_t)part * a.Out * a.in.n;
+    if (bias) db += (size_t)part * a.Out;
+  }
+  float c[TM], sum[TM];
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    c[m] = sums.offset[m] + __shfl_xor(sums.offset[m], 32, 64);
+    sum[m] = sums.bias[m] + __shfl_xor(sums.bias[m], 32, 64);
+    if (KW > 1 && kw == 1 && half == 0) {
+      halves[0][wave][m][r] = c[m];
+      halves[KW > 1 ? 1 : 0][wave][m][r] = sum[m];
+    }
+  }
+  if (KW > 1) {
+    // each group hands the other two of its four column tiles: 32 values per thread and row tile, through the columns' memory
+    float *swap = reinterpret_cast<float *>(&cols[0][0][0][0]);
+    const uint32_t tid = threadIdx.x % THREADS;
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      __syncthreads();  // the columns, or the values of the row tile before, are no longer read
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) swap[(kw * 32u + n * 16u + i) * THREADS + tid] = kw == 0 ? sums.acc[m][n + 2][i] : sums.acc[m][n][i];
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float other = swap[((kw ^ 1u) * 32u + n * 16u + i) * THREADS + tid];
+          if (kw == 0)
+            sums.acc[m][n][i] += other;
+          else
+            sums.acc[m][n + 2][i] = other + sums.acc[m][n + 2][i];
+        }
+    }
+  }
+  if (kw == 0 && half == 0) {
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      if (KW > 1) {
+        c[m] += halves[0][wave][m][r];
+        sum[m] += halves[KW > 1 ? 1 : 0][wave][m][r];
+      }
+      reinterpret_cast<float *>(offsets[wave][m])[r] = c[m];
+      if (bias && m0 + r * TM + m < a.Out) {
+        float *p = db + m0 + r * TM + m;
+        *p = a.accumulate ? *p + sum[m] : sum[m];
+      }
+    }
+  }
+  __syncthreads();
+  if constexpr (KW == 1) {
+    packed_wgrad_store<TM, 0, 4>(a, dw, g, m0, offsets[wave], sums);
+  } else if (kw == 0) {
+    packed_wgrad_store<TM, 0, 2>(a, dw, g, m0, offsets[wave], sums);
+  } else {
+    packed_wgrad_store<TM, 2, 4>(a, dw, g, m0, offsets[wave], sums);
+  }
+}
+
+// the parts of a split sum, in a fixed order: first the weights' n values, then the bias's Out; SLICES threads per value, which take
+// every SLICES-th part
+template <int SLICES>
 __global__ __launch_bounds__(THREADS) void packed_wgrad_join_kernel(float *dweight, float *dbias, const float *partial, const float *partial_bias, uint32_t split, size_t n,
                                                                    uint32_t Out, bool accumulate) {
-  const size_t i = (size_t)blockIdx.x * THREADS + threadIdx.x;
-  const bool weight = i < n;
-  if (!weight && (dbias == nullptr || i - n >= Out)) return;
+  constexpr uint32_t VALUES = THREADS / SLICES;
+  __shared__ float sums[SLICES][VALUES];
+  const uint32_t c = threadIdx.x % VALUES, slice = threadIdx.x / VALUES;
+  const size_t i = (size_t)blockIdx.x * VALUES + c;
+  const bool weight = i < n, exists = weight || (dbias != nullptr && i - n < Out);
   const float *p = weight ? partial + i : partial_bias + (i - n);
-  float *out = weight ? dweight + i : dbias + (i - n);
   const size_t stride = weight ? n : Out;
   float s = 0.f;
-#pragma unroll 4
-  for (uint32_t k = 0; k < split; k++, p += stride) s += *p;
+  if (exists)
+    for (uint32_t k = slice; k < split; k += 8 * SLICES) {
+      float t[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) t[u] = k + u * SLICES < split ? p[(size_t)(k + u * SLICES) * stride] : 0.f;
+      s += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+    }
+  if (SLICES > 1) {
+    sums[slice][c] = s;
+    __syncthreads();
+    if (slice != 0) return;
+#pragma unroll
+    for (int k = 1; k < SLICES; k++) s += sums[k][c];
+  }
+  if (!exists) return;
+  float *out = weight ? dweight + i : dbias + (i - n);
   *out = accumulate ? *out + s : s;
 }
 
@@ -262,6 +337,40 @@ __global__ __launch_bounds__(THREADS) void bias_only_kernel(float *dbias, const 
 }
 
 mt::Workspace g_wgrad_ws;
+
+// The variant: rows per block (256: each sample's columns are turned into bf16 for twice the products; 128: twice the blocks), one or
+// two groups of wavefronts per block, parts of the batch.  The estimate of each variant's time in microseconds is its fixed part plus
+// the steps that the busiest compute unit takes, at the measured time of a step with one or two blocks on it, plus writing and
+// joining the parts' sums.  Measured against one another: 4096^3 366 us with 256 rows, 412 with 128; 2048^3 58 with 128 rows and
+// two groups, 66 with one, 72 with 256 rows and four parts; 1000 x 1000 x 1777 27.5 with two groups, 31.9 with two parts; 512^3 11.2 in
+// four parts, 19 in one.
+struct Plan {
+  uint32_t rows, split;
+  bool pair;
+};
+Plan choose(uint32_t Out, uint32_t groups, uint32_t steps, size_t n) {
+  Plan best{128, 1, false};
+  double least = 1e30;
+  for (int kind = 0; kind < 3; kind++) {
+    const uint32_t rows = kind == 2 ? 256 : 128;
+    const bool pair = kind == 1;
+    if (rows == 256 && Out % 2 != 0) continue;  // rows are loaded in pairs there, which must not straddle the end
+    const double fixed = kind == 0 ? 5.0 : kind == 1 ? 6.0 : 6.5, one = kind == 0 ? 1.75 : kind == 1 ? 3.0 : 2.8, two = kind == 0 ? 3.25 : kind == 1 ? 6.0 : 5.7;
+    const size_t tiles = (size_t)cdiv(Out, rows) * groups;
+    for (uint32_t split = 1; split <= 128 && split <= steps; split += split < 4 ? 1 : split / 2) {
+      const size_t blocks = tiles * split;
+      const size_t rest = blocks % 512;
+      const double turn = blocks / 512 * two + (rest > 256 ? two : rest > 0 ? one : 0.0);
+      const uint32_t each = cdiv(cdiv(steps, split), pair ? 2 : 1);
+      const double us = fixed + each * turn + (split > 1 ? 4.0 + split * (double)n * 2e-6 : 0.0);
+      if (us < least) {
+        least = us;
+        best = Plan{rows, split, pair};
+      }
+    }
+  }
+  return best;
+}
 
 }  // namespace
 
@@ -299,20 +408,15 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   }
   WgradArgs a{};
   a.delta = delta->p; a.in = v; a.Out = Out; a.accumulate = accumulate != 0;
-  const bool wide = Out % 2 == 0 && Out > 128 && (size_t)cdiv(Out, 256) * v.groups * cdiv(v.w, 1024) >= 256;
-  a.tiles_m = cdiv(Out, wide ? 256 : 128);
+  const size_t n = (size_t)Out * v.n;
+  const uint32_t steps = cdiv(v.w, KSTEP);
+  const Plan plan = choose(Out, v.groups, steps, n);
+  const bool wide = plan.rows == 256, pair = plan.pair;
+  const uint32_t split = plan.split;
+  a.tiles_m = cdiv(Out, plan.rows);
   const size_t tiles = (size_t)a.tiles_m * v.groups;
-  // few tiles: parts of the batch, at least 256 samples each, until the chip has its two blocks per compute unit
-  uint32_t split = 1;
-  if (tiles < 512) {
-    split = (uint32_t)(512 / tiles);
-    const uint32_t most = v.w / 256;
-    if (split > most) split = most;
-    if (split < 1) split = 1;
-  }
   a.per_split = cdiv(cdiv(v.w, split), KSTEP) * KSTEP;
   a.split = cdiv(v.w, a.per_split);
-  const size_t n = (size_t)Out * v.n;
   float *ws = nullptr;
   if (a.split > 1) {
     int rc = mt::workspace_get(g_wgrad_ws, "packed weight gradient", a.split * (n + Out), &ws);
@@ -327,12 +431,18 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   const size_t grid = tiles * a.split;
   if (grid > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);
   if (wide)
-    packed_wgrad_kernel<2><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+    packed_wgrad_kernel<2, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  else if (pair)
+    packed_wgrad_kernel<1, 2><<<(unsigned)grid, 2 * THREADS, 0, mt::stream()>>>(a);
   else
-    packed_wgrad_kernel<1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+    packed_wgrad_kernel<1, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
   MT_LAUNCH_CHECK(name);
   if (a.split > 1) {
-    packed_wgrad_join_kernel<<<cdiv(n + Out, THREADS), THREADS, 0, mt::stream()>>>(dweight->p, dbias ? dbias->p : nullptr, ws, ws + a.split * n, a.split, n, Out, accumulate != 0);
+    float *db = dbias ? dbias->p : nullptr;
+    if (a.split > 8)
+      packed_wgrad_join_kernel<4><<<cdiv(n + Out, THREADS / 4), THREADS, 0, mt::stream()>>>(dweight->p, db, ws, ws + a.split * n, a.split, n, Out, accumulate != 0);
+    else
+      packed_wgrad_join_kernel<1><<<cdiv(n + Out, THREADS), THREADS, 0, mt::stream()>>>(dweight->p, db, ws, ws + a.split * n, a.split, n, Out, accumulate != 0);
     MT_LAUNCH_CHECK(name);
   }
   return MT_OK;

@@ -491,11 +491,11 @@ class CTensorMath:
     # ---- activations in 8 bits (no counterpart in the reference)
     @staticmethod
     def Pack(out, inp):
-        call("mt_pack", _d(out), _d(inp))
+        call("mt_pack", out.ref(), inp.ref())
 
     @staticmethod
     def Unpack(out, inp):
-        call("mt_unpack", _d(out), _d(inp))
+        call("mt_unpack", out.ref(), inp.ref())
 
     @staticmethod
     def CreateDropOutMatrix(out, drop_out, seed):
@@ -623,24 +623,20 @@ class Fused:
     def LayerNormForward(out, inp, gamma, beta, mean=None, ivar=None, packed=None, epsilon=1e-6, func=None):
         """Rows as gamma names them ([1,Z,Y,X], [1,1,Y,X] or [1,1,1,X]) normalised by their own statistics.  mean, ivar: kept for
         the backward pass; packed: a CPackedTensor that receives the input in 8 bits."""
-        opt = lambda t: _d(t) if t is not None else None
-        call("mt_layernorm_forward_func", _d(out), _d(inp), _d(gamma), _d(beta), opt(mean), opt(ivar), opt(packed), _f(epsilon), C.c_int(FUNC[func]))
+        call("mt_layernorm_forward_func", out.ref(), inp.ref(), gamma.ref(), beta.ref(), mean and mean.ref(), ivar and ivar.ref(), packed and packed.ref(),
+             _f(epsilon), FUNC[func])
 
     @staticmethod
     def LayerNormBackward(error, dgamma, dbeta, delta, gamma, inp, mean, ivar, beta=None, func=None, accumulate=True):
         """inp: the forward pass's input, as a CTensor or as the CPackedTensor that it left.  accumulate: dgamma and dbeta are added
         to (as the other backward calls do) or overwritten."""
-        opt = lambda t: _d(t) if t is not None else None
-        args = (_d(error), opt(dgamma), opt(dbeta), _d(delta), _d(gamma), opt(beta), _d(inp), _d(mean), _d(ivar), C.c_int(FUNC[func]), C.c_int(1 if accumulate else 0))
-        if isinstance(inp, CPackedTensor):
-            call("mt_layernorm_backward_packed_func", *args)
-        else:
-            call("mt_layernorm_backward_func", *args)
+        call("mt_layernorm_backward_packed_func" if isinstance(inp, CPackedTensor) else "mt_layernorm_backward_func", error.ref(), dgamma and dgamma.ref(),
+             dbeta and dbeta.ref(), delta.ref(), gamma.ref(), beta and beta.ref(), inp.ref(), mean.ref(), ivar.ref(), FUNC[func], 1 if accumulate else 0)
 
     @staticmethod
     def LinearBackwardWeightsSum(dweight, dbias, inp, delta, accumulate=True):
         """Weight and bias gradient of a linear layer, summed over the batch, from its input kept in 8 bits (a CPackedTensor)."""
-        call("mt_linear_backward_weights_sum_packed", _d(dweight), _d(dbias) if dbias is not None else None, _d(inp), _d(delta), C.c_int(1 if accumulate else 0))
+        call("mt_linear_backward_weights_sum_packed", dweight.ref(), dbias and dbias.ref(), inp.ref(), delta.ref(), 1 if accumulate else 0)
 
     @staticmethod
     def BatchNormForwardInfer(out, inp, gamma, beta, mean, variable, epsilon=1e-6, func=None):

@@ -1214,6 +1214,7 @@ __global__ __launch_bounds__(EW_THREADS) void bn_scale_shift_kernel(float2 *ss, 
 }  // namespace
 
 namespace mt {
+bool past_caches(size_t bytes) { return streamed(bytes); }
 int set_nontemporal(int v) {
   if (v < 0 || v > 2) return fail(MT_E_ARGUMENT, "nontemporal must be 0 (never), 1 (always) or 2 (tensors of 128 MiB and more)");
   g_nontemporal = v;

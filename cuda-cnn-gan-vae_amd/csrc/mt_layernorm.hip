@@ -58,44 +58,50 @@ __device__ __forceinline__ void apply(int func, float *v) {
   }
 }
 
+// ---- one step of a thread: one value, four neighbouring ones, or four past the caches, for tensors that are too large for them and
+// touched once (option "nontemporal": 128 MiB and more; 16384 x 4096 forward 102 -> 98 us, backward 148 -> 139).  A flag at run time does
+// not do: the compiler merges the two accesses into the ordinary one. -----------------------------------------------------------
+enum Access { ONE, FOUR, FOUR_PAST };
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+template <int ACCESS>
+__device__ __forceinline__ void load_step(float *t, const float *p, uint32_t at) {
+  if (ACCESS == ONE) {
+    t[0] = p[at];
+  } else {
+    const floatx4 *q = reinterpret_cast<const floatx4 *>(p + at);
+    const floatx4 v = ACCESS == FOUR_PAST ? __builtin_nontemporal_load(q) : *q;
+    t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
+  }
+}
+template <int ACCESS>
+__device__ __forceinline__ void store_step(float *p, const float *t) {
+  if (ACCESS == ONE) {
+    *p = t[0];
+  } else {
+    const floatx4 v = {t[0], t[1], t[2], t[3]};
+    if (ACCESS == FOUR_PAST)
+      __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(p));
+    else
+      *reinterpret_cast<floatx4 *>(p) = v;
+  }
+}
+
 // ---- how the L threads of a row share its N values: E each, in vectors of four 4 * L apart, or singly L apart ----------------
 template <int L, int E, bool VEC>
 struct Share {
   static constexpr int STEPS = VEC ? E / 4 : E, WIDTH = VEC ? 4 : 1;
   static __device__ __forceinline__ uint32_t first(int j) { return (j * L + threadIdx.x % L) * WIDTH; }
-  // values behind the end read the last ones again and count as `other`
-  static __device__ __forceinline__ void load(float (&v)[E], const float *p, uint32_t N, float other) {
+  // values behind the end read the last ones again and count as 0
+  template <int ACCESS = VEC ? FOUR : ONE>
+  static __device__ __forceinline__ void load(float (&v)[E], const float *p, uint32_t N) {
 #pragma unroll
-    for (int j = 0; j < STEPS; j++) {
-      const uint32_t i = first(j), at = min(i, N - WIDTH);
-      if (VEC) {
-        const float4 t = *reinterpret_cast<const float4 *>(p + at);
-        v[j * WIDTH] = t.x; v[j * WIDTH + WIDTH / 4] = t.y; v[j * WIDTH + WIDTH / 2] = t.z; v[j * WIDTH + WIDTH - 1] = t.w;
-      } else {
-        v[j] = p[at];
-      }
-    }
+    for (int j = 0; j < STEPS; j++) load_step<ACCESS>(v + j * WIDTH, p, min(first(j), N - WIDTH));
 #pragma unroll
     for (int j = 0; j < STEPS; j++)
 #pragma unroll
-      for (int e = 0; e < WIDTH; e++) v[j * WIDTH + e] = first(j) < N ? v[j * WIDTH + e] : other;
-  }
-  static __device__ __forceinline__ void store(float *p, int j, const float *t) {
-    if (VEC)
-      *reinterpret_cast<float4 *>(p + first(j)) = make_float4(t[0], t[WIDTH / 4], t[WIDTH / 2], t[WIDTH - 1]);
-    else
-      p[first(j)] = t[0];
+      for (int e = 0; e < WIDTH; e++) v[j * WIDTH + e] = first(j) < N ? v[j * WIDTH + e] : 0.f;
   }
 };
-template <bool VEC>
-__device__ __forceinline__ void load_step(float *t, const float *p, uint32_t at) {
-  if (VEC) {
-    const float4 q = *reinterpret_cast<const float4 *>(p + at);
-    t[0] = q.x; t[1] = q.y; t[2] = q.z; t[3] = q.w;
-  } else {
-    t[0] = p[at];
-  }
-}
 
 // ---- where a row's input comes from in the backward pass: the fp32 tensor, or the 8 bits the forward pass kept.  Loading and
 // decoding are two steps, so that all loads of a row are under way before the first is waited for ------------------------------
@@ -112,8 +118,8 @@ struct RowsF32 {
   };
   struct Row {
     const float *p;
-    template <bool VEC>
-    __device__ __forceinline__ void load(Raw<VEC> &raw, uint32_t at) const { load_step<VEC>(raw.t, p, at); }
+    template <int ACCESS>
+    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, uint32_t at) const { load_step<ACCESS>(raw.t, p, at); }
   };
   __device__ __forceinline__ Row row(uint32_t r) const { return Row{p + (size_t)r * N}; }
 };
@@ -133,11 +139,11 @@ struct RowsPacked {
     const uint8_t *q;
     const float2 *pair;
     uint32_t first;  // the row's first value within its sample
-    template <bool VEC>
-    __device__ __forceinline__ void load(Raw<VEC> &raw, uint32_t at) const {
+    template <int ACCESS>
+    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, uint32_t at) const {
       const uint32_t e = first + at;
       raw.pair = pair[e / mt::PACK_GROUP];
-      raw.q = VEC ? *reinterpret_cast<const uint32_t *>(q + e) : q[e];
+      raw.q = ACCESS != ONE ? *reinterpret_cast<const uint32_t *>(q + e) : q[e];
     }
   };
   __device__ __forceinline__ Row row(uint32_t r) const {
@@ -172,32 +178,34 @@ struct Forward {
 };
 
 // gamma * xhat + beta and the function, from x in registers
-template <int L, int E, bool VEC>
+template <int L, int E, int ACCESS>
 __device__ __forceinline__ void normalise(const Forward &a, float *out, const float (&x)[E], float mean, float ivar, const float *gamma, const float *beta, uint32_t N) {
+  constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, VEC>;
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) {
     if (S::first(j) >= N) continue;
     float g[S::WIDTH], b[S::WIDTH], y[S::WIDTH];
-    load_step<VEC>(g, gamma, S::first(j));
-    load_step<VEC>(b, beta, S::first(j));
+    load_step<VEC ? FOUR : ONE>(g, gamma, S::first(j));
+    load_step<VEC ? FOUR : ONE>(b, beta, S::first(j));
 #pragma unroll
     for (int e = 0; e < S::WIDTH; e++) y[e] = g[e] * ((x[j * S::WIDTH + e] - mean) * ivar) + b[e];
     apply<S::WIDTH>(a.func, y);
-    S::store(out, j, y);
+    store_step<ACCESS>(out + S::first(j), y);
   }
 }
 
 // rows that fit the registers of L threads
-template <int L, int E, bool VEC, bool PACK>
+template <int L, int E, int ACCESS, bool PACK>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a) {
+  constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
   __shared__ float part[2][L / 64 + 1];
   const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
   const bool mine = want < a.rows;
   float x[E];
-  S::load(x, a.in + (size_t)row * a.N, a.N, 0.f);
+  S::template load<ACCESS>(x, a.in + (size_t)row * a.N, a.N);
   if (PACK) {
     const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N;
 #pragma unroll
@@ -218,7 +226,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a
     }
   const float ivar = 1.f / sqrtf(row_sum<L>(s, part[1]) / (float)a.N + a.eps);
   if (!mine) return;
-  normalise<L, E, VEC>(a, a.out + (size_t)row * a.N, x, mean, ivar, a.gamma, a.beta, a.N);
+  normalise<L, E, ACCESS>(a, a.out + (size_t)row * a.N, x, mean, ivar, a.gamma, a.beta, a.N);
   if (threadIdx.x % L == 0) {
     if (a.mean) a.mean[row] = mean;
     if (a.ivar) a.ivar[row] = ivar;
@@ -233,7 +241,7 @@ __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *s
   __shared__ float part[2][THREADS / 64];
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE);
   float x[PIECE / THREADS];
-  S::load(x, a.in + (size_t)row * a.N + (size_t)piece * PIECE, n, 0.f);
+  S::load(x, a.in + (size_t)row * a.N + (size_t)piece * PIECE, n);
   if (PACK) {
     const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N + piece * PIECE;
 #pragma unroll
@@ -256,13 +264,14 @@ __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *s
 }
 // ... then every block joins the pieces of its row (each wavefront for itself: the sum of deviations of a piece moves by
 // n * (its mean - the row's mean)^2) and normalises its own piece
-template <bool VEC>
+template <int ACCESS>
 __global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const float2 *stats, uint32_t pieces) {
+  constexpr bool VEC = ACCESS != ONE;
   using S = Share<THREADS, PIECE / THREADS, VEC>;
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, lane = threadIdx.x % 64, n = min(PIECE, a.N - piece * PIECE);
   const size_t at = (size_t)row * a.N + (size_t)piece * PIECE;
   float x[PIECE / THREADS];
-  S::load(x, a.in + at, n, 0.f);
+  S::template load<ACCESS>(x, a.in + at, n);
   stats += (size_t)row * pieces;
   float s = 0.f;
   for (uint32_t p = lane; p < pieces; p += 64) s += stats[p].x * (float)min(PIECE, a.N - p * PIECE);
@@ -274,7 +283,7 @@ __global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const floa
     s += t.y + d * d * (float)min(PIECE, a.N - p * PIECE);
   }
   const float ivar = 1.f / sqrtf(mt::over_lanes<mt::Sum, 64>(s) / (float)a.N + a.eps);
-  normalise<THREADS, PIECE / THREADS, VEC>(a, a.out + at, x, mean, ivar, a.gamma + (size_t)piece * PIECE, a.beta + (size_t)piece * PIECE, n);
+  normalise<THREADS, PIECE / THREADS, ACCESS>(a, a.out + at, x, mean, ivar, a.gamma + (size_t)piece * PIECE, a.beta + (size_t)piece * PIECE, n);
   if (piece == 0 && threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
     if (a.ivar) a.ivar[row] = ivar;
@@ -350,8 +359,9 @@ __global__ __launch_bounds__(SLICES == 1 ? THREADS : 64 * SLICES) void ln_join_k
 }
 
 // rows that fit the registers of L threads; a block walks over the rows and keeps its share of dgamma and dbeta in registers
-template <int L, int E, bool VEC, bool FUNC, class Rows>
+template <int L, int E, int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
+  constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
   constexpr int W = S::WIDTH;
@@ -361,8 +371,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
   constexpr bool HELD = L < 1024;  // gamma and beta stay in registers; 1024 threads load them for every row
   float dg[E], db[E], gamma[E], beta[FUNC ? E : 1];
   const auto load_parameters = [&] {
-    S::load(gamma, a.gamma, a.N, 0.f);
-    if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
+    S::load(gamma, a.gamma, a.N);
+    if constexpr (FUNC) S::load(beta, a.beta, a.N);
   };
   if constexpr (HELD) load_parameters();
 #pragma unroll
@@ -380,9 +390,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     *m = a.mean[row];
     *v = a.ivar[row];
     const auto in = rows.row(row);
-    S::load(gr, a.delta + (size_t)row * a.N, a.N, 0.f);
+    S::template load<ACCESS>(gr, a.delta + (size_t)row * a.N, a.N);
 #pragma unroll
-    for (int j = 0; j < S::STEPS; j++) in.load(r[j], min(S::first(j), a.N - W));
+    for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(r[j], min(S::first(j), a.N - W));
   };
   if constexpr (EARLY) load(min(blockIdx.x * PER_BLOCK + sub, a.rows - 1), raw, g, &mean, &ivar);
   for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += stride, turn ^= 1u) {
@@ -443,7 +453,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
         float t[W];
 #pragma unroll
         for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
-        S::store(error, j, t);
+        store_step<ACCESS>(error + S::first(j), t);
       }
     }
     if constexpr (EARLY) {
@@ -460,8 +470,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 #pragma unroll
     for (int j = 0; j < S::STEPS; j++)
       if (S::first(j) < a.N) {
-        S::store(pg, j, dg + j * W);
-        S::store(pb, j, db + j * W);
+        store_step<VEC ? FOUR : ONE>(pg + S::first(j), dg + j * W);
+        store_step<VEC ? FOUR : ONE>(pb + S::first(j), db + j * W);
       }
     return;
   }
@@ -490,8 +500,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 // The error alone, one row per L threads, and beside it in the same launch (blocks from error_blocks on) dgamma and dbeta straight
 // from delta and x: they need no sum over a row.  That reads both a second time, from the caches, where the kernel above writes and
 // joins partial sums: 256 rows of 4096 10.7 -> 5.2 us, 33 of 1001 7.0 -> 4.9; 8192 of 2048 would lose (36 us against 50).
-template <int L, int E, bool VEC, bool FUNC, class Rows>
+template <int L, int E, int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t error_blocks) {
+  constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
   constexpr int W = S::WIDTH;
@@ -510,7 +521,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
       for (int u = 0; u < 4; u++) {
         const uint32_t row = min(k + 16 * u, a.rows - 1);
         g[u] = a.delta[(size_t)row * a.N + i];
-        rows.row(row).load(raw[u], i);
+        rows.row(row).template load<ONE>(raw[u], i);
         mean[u] = a.mean[row];
         ivar[u] = a.ivar[row];
       }
@@ -547,11 +558,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
   const auto in = rows.row(row);
   typename Rows::template Raw<VEC> raw[S::STEPS];
   float x[E], g[E], gamma[E], beta[FUNC ? E : 1];
-  S::load(g, a.delta + (size_t)row * a.N, a.N, 0.f);
+  S::template load<ACCESS>(g, a.delta + (size_t)row * a.N, a.N);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.load(raw[j], min(S::first(j), a.N - W));
-  S::load(gamma, a.gamma, a.N, 0.f);
-  if constexpr (FUNC) S::load(beta, a.beta, a.N, 0.f);
+  for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(raw[j], min(S::first(j), a.N - W));
+  S::load(gamma, a.gamma, a.N);
+  if constexpr (FUNC) S::load(beta, a.beta, a.N);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
@@ -578,7 +589,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
     float t[W];
 #pragma unroll
     for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
-    S::store(a.error + (size_t)row * a.N, j, t);
+    store_step<ACCESS>(a.error + (size_t)row * a.N + S::first(j), t);
   }
 }
 
@@ -593,12 +604,12 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
   const auto in = rows.row(row);
   typename Rows::template Raw<VEC> raw[S::STEPS];
   float x[PIECE / THREADS], g[PIECE / THREADS];
-  S::load(g, a.delta + (size_t)row * a.N + at, n, 0.f);
+  S::load(g, a.delta + (size_t)row * a.N + at, n);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.load(raw[j], at + min(S::first(j), n - W));
+  for (int j = 0; j < S::STEPS; j++) in.template load<VEC ? FOUR : ONE>(raw[j], at + min(S::first(j), n - W));
   float gamma[PIECE / THREADS], beta[FUNC ? PIECE / THREADS : 1];
-  S::load(gamma, a.gamma + at, n, 0.f);
-  if constexpr (FUNC) S::load(beta, a.beta + at, n, 0.f);
+  S::load(gamma, a.gamma + at, n);
+  if constexpr (FUNC) S::load(beta, a.beta + at, n);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
@@ -621,9 +632,10 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
 }
 // ... then blocks of 256 * WIDTH columns that walk over a group of rows: the error, and their columns' share of dgamma and dbeta
 constexpr uint32_t GROUP_ROWS = 64;  // rows of a group, at most
-template <bool VEC, bool FUNC, class Rows>
+template <int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a, Rows rows, const float2 *sums, uint32_t pieces, uint32_t groups, uint32_t per_group,
                                                                      float *partial) {
+  constexpr bool VEC = ACCESS != ONE;
   constexpr int W = VEC ? 4 : 1;
   __shared__ float4 terms[GROUP_ROWS];  // of each row: mean, ivar, sum(u) / N, sum(u * xhat) / N
   const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * THREADS + threadIdx.x) * W, at = min(column, a.N - W);
@@ -644,8 +656,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
   float gamma[AT_ONCE][W], beta[AT_ONCE][W], dg[W] = {}, db[W] = {};
 #pragma unroll
   for (uint32_t u = 0; u < AT_ONCE; u++) {
-    load_step<VEC>(gamma[u], a.gamma, at);
-    if (FUNC) load_step<VEC>(beta[u], a.beta, at);
+    load_step<VEC ? FOUR : ONE>(gamma[u], a.gamma, at);
+    if (FUNC) load_step<VEC ? FOUR : ONE>(beta[u], a.beta, at);
   }
   __syncthreads();
   // four rows at a time, loaded before the first of them is stored (the error may be written over delta: each thread reads and
@@ -656,8 +668,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
       const uint32_t row = first + min(k0 + u, count - 1);
-      load_step<VEC>(g[u], a.delta + (size_t)row * a.N, at);
-      rows.row(row).load(raw[u], at);
+      load_step<ACCESS>(g[u], a.delta + (size_t)row * a.N, at);
+      rows.row(row).template load<ACCESS>(raw[u], at);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -680,11 +692,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
         t[e] = c.y * ((g[u][e] * gamma[u][e] - c.z) - x[u][e] * c.w);
       }
       if (column < a.N) {
-        float *p = a.error + (size_t)(first + k0 + u) * a.N + column;
-        if (VEC)
-          *reinterpret_cast<float4 *>(p) = make_float4(t[0], t[W / 4], t[W / 2], t[W - 1]);
-        else
-          *p = t[0];
+        store_step<ACCESS>(a.error + (size_t)(first + k0 + u) * a.N + column, t);
       }
     }
   }
@@ -716,7 +724,7 @@ __global__ __launch_bounds__(THREADS) void ln_front_kernel(Backward a, Rows rows
     for (uint32_t i = blockIdx.y * THREADS + threadIdx.x; i < a.N; i += gridDim.y * THREADS) {
       typename Rows::template Raw<false> raw;
       float x;
-      in.load(raw, i);
+      in.template load<ONE>(raw, i);
       raw.values(&x);
       const size_t e = (size_t)row * a.N + i;
       a.error[e] = a.delta[e] * mt::apply_func(MT_F_DIFFERENTIAL + a.func, a.gamma[i] * ((x - mean) * ivar) + a.beta[i]);
@@ -766,18 +774,23 @@ bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { 
 constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384, BACKWARD_ROW_TIGHT = 8192;
 
 template <int L, int E>
-void forward_rows(const Forward &a, bool vec, bool pack) {
+void forward_rows(const Forward &a, int access, bool pack) {
   const unsigned grid = cdiv(a.rows, L < 256 ? 256 / L : 1), threads = L < 256 ? 256 : L;
   if constexpr (L >= 64) {
     if (pack) {
-      ln_forward_kernel<L, E, true, true><<<grid, threads, 0, mt::stream()>>>(a);
+      if (access == FOUR_PAST)
+        ln_forward_kernel<L, E, FOUR_PAST, true><<<grid, threads, 0, mt::stream()>>>(a);
+      else
+        ln_forward_kernel<L, E, FOUR, true><<<grid, threads, 0, mt::stream()>>>(a);
       return;
     }
   }
-  if (vec)
-    ln_forward_kernel<L, E, true, false><<<grid, threads, 0, mt::stream()>>>(a);
+  if (access == FOUR_PAST)
+    ln_forward_kernel<L, E, FOUR_PAST, false><<<grid, threads, 0, mt::stream()>>>(a);
+  else if (access == FOUR)
+    ln_forward_kernel<L, E, FOUR, false><<<grid, threads, 0, mt::stream()>>>(a);
   else
-    ln_forward_kernel<L, E, false, false><<<grid, threads, 0, mt::stream()>>>(a);
+    ln_forward_kernel<L, E, ONE, false><<<grid, threads, 0, mt::stream()>>>(a);
 }
 
 // calls f with the threads per row and the values per thread that hold a row of N values
@@ -799,14 +812,18 @@ int with_share(uint32_t N, F &&f) {
   return f(integral_constant<int, 1024>{}, integral_constant<int, 32>{});
 }
 
-// calls f with what a kernel is compiled for
+// calls f with what a kernel is compiled for: how it accesses the tensors, whether a function stands behind the norm
 template <class F>
-void with_kind(bool vec, bool func, F &&f) {
-  if (vec) {
-    if (func) f(std::true_type{}, std::true_type{}); else f(std::true_type{}, std::false_type{});
-  } else {
-    if (func) f(std::false_type{}, std::true_type{}); else f(std::false_type{}, std::false_type{});
-  }
+void with_kind(int access, bool func, F &&f) {
+  const auto with_access = [&](auto acc) {
+    if (func) f(acc, std::true_type{}); else f(acc, std::false_type{});
+  };
+  if (access == FOUR_PAST)
+    with_access(std::integral_constant<int, FOUR_PAST>{});
+  else if (access == FOUR)
+    with_access(std::integral_constant<int, FOUR>{});
+  else
+    with_access(std::integral_constant<int, ONE>{});
 }
 
 template <class Rows>
@@ -825,6 +842,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
   }
   const bool params = dgamma || dbeta;
   const bool vec = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
+  const int access = !vec ? ONE : mt::past_caches(mt::count(delta) * 4) ? FOUR_PAST : FOUR;
   // few rows: the parameter gradients beside the error instead of partial sums and their join
   const bool few = g.rows <= 512;
   uint32_t parts = 0;
@@ -838,7 +856,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         if (beside) {
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
           const auto go = [&](uint32_t grid, uint32_t first_param_block) {
-            with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
+            with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
               ln_backward_few_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
             });
           };
@@ -858,8 +876,10 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         if (parts > most) parts = most;
         int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
         if (rc) return rc;
-        with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
-          ln_backward_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+        with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
+          constexpr int ACCESS = decltype(v)::value;
+          constexpr bool FUNC = decltype(f)::value;
+          if constexpr (L * E <= (int)BACKWARD_ROW_TIGHT || (ACCESS != ONE && !FUNC)) ln_backward_kernel<L, E, ACCESS, FUNC, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
         });
       }
       return (int)MT_OK;
@@ -883,10 +903,11 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     float2 *piece_sums = reinterpret_cast<float2 *>(ws);
     partial = ws + sums;
     parts = groups > 1 ? groups : 0;
-    with_kind(vec, a.func != MT_F_NONE, [&](auto v, auto f) {
-      constexpr bool VEC = decltype(v)::value, FUNC = decltype(f)::value;
-      ln_backward_pieces_kernel<VEC, FUNC><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
-      ln_backward_columns_kernel<VEC, FUNC><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
+    with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
+      constexpr int ACCESS = decltype(v)::value;
+      constexpr bool FUNC = decltype(f)::value;
+      ln_backward_pieces_kernel<ACCESS != ONE, FUNC><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
+      ln_backward_columns_kernel<ACCESS, FUNC><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
     });
     MT_LAUNCH_CHECK(name);
   }
@@ -969,6 +990,7 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
   a.packed = packed; a.rows = g.rows; a.N = g.N; a.per_sample = g.per_sample; a.eps = epsilon;
   a.func = func == MT_F_GELU ? MT_F_NONE : func;  // GeLU (double arithmetic, a library function) runs over the output afterwards
   const bool vec = g.N % 4 == 0 && aligned16(a.out) && aligned16(a.in) && aligned16(a.gamma) && aligned16(a.beta);
+  const int access = !vec ? ONE : mt::past_caches(mt::count(in) * 4) ? FOUR_PAST : FOUR;
   // the same pass can leave the 8 bits where a row starts at a group's first value and 32 lanes hold a group
   const bool pack = packed_input && vec && g.N > 128 && (g.N % mt::PACK_GROUP == 0 || g.per_sample == 1);
   if (packed_input && !pack && (rc = mt_pack(packed_input, in))) return rc;
@@ -977,7 +999,7 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
     mt::ProfileScope prof(name);
     if (g.N <= FORWARD_ROW) {
       rc = with_share(g.N, [&](auto l, auto e) {
-        forward_rows<decltype(l)::value, decltype(e)::value>(a, vec, pack);
+        forward_rows<decltype(l)::value, decltype(e)::value>(a, access, pack);
         return (int)MT_OK;
       });
       MT_LAUNCH_CHECK(name);
@@ -995,10 +1017,7 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
       else
         ln_pieces_kernel<false, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
       MT_LAUNCH_CHECK(name);
-      if (vec)
-        ln_apply_kernel<true><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
-      else
-        ln_apply_kernel<false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      with_kind(access, false, [&](auto v, auto) { ln_apply_kernel<decltype(v)::value><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces); });
       MT_LAUNCH_CHECK(name);
     }
   }

@@ -14,6 +14,8 @@ constexpr int AT_ONCE = 4;   // groups in flight per 32 lanes
 // Both kernels move 5 bytes per value and compute little: what they need is enough loads in flight.  32 lanes take a group, four
 // values each (one 128-bit access where the tensor allows, four values 32 apart otherwise), and work on four groups at once.
 // Samples of whole groups are one long row of groups (`rows` false): no division by the groups of a sample is needed then.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
 struct PackJob {
   PackedView v;
   uint64_t total;  // groups of the whole tensor
@@ -34,7 +36,7 @@ __device__ __forceinline__ Place place(const PackJob &job, uint64_t g) {
 template <bool VEC>
 __device__ __forceinline__ uint32_t within(uint32_t lane, int k) { return VEC ? lane * 4u + k : lane + 32u * k; }
 
-template <bool VEC, class Index>
+template <bool VEC, bool PAST, class Index>
 __global__ __launch_bounds__(THREADS) void pack_kernel(PackJob job, const float *in) {
   const uint32_t lane = threadIdx.x % LANES;
   const uint64_t step = (uint64_t)gridDim.x * (THREADS / LANES);
@@ -46,7 +48,8 @@ __global__ __launch_bounds__(THREADS) void pack_kernel(PackJob job, const float 
       const uint64_t g = g0 + u * step < job.total ? g0 + u * step : g0;
       at[u] = place<Index>(job, g);
       if (VEC) {
-        const float4 t = *reinterpret_cast<const float4 *>(in + at[u].tensor + min(lane * 4u, at[u].count - 4u));  // behind the end: values of the group again
+        const floatx4 *p = reinterpret_cast<const floatx4 *>(in + at[u].tensor + min(lane * 4u, at[u].count - 4u));  // behind the end: values of the group again
+        const floatx4 t = PAST ? __builtin_nontemporal_load(p) : *p;
         v[u][0] = t.x; v[u][1] = t.y; v[u][2] = t.z; v[u][3] = t.w;
       } else {
 #pragma unroll
@@ -75,7 +78,7 @@ __global__ __launch_bounds__(THREADS) void pack_kernel(PackJob job, const float 
   }
 }
 
-template <bool VEC, class Index>
+template <bool VEC, bool PAST, class Index>
 __global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackJob job) {
   const uint32_t lane = threadIdx.x % LANES;
   const uint64_t step = (uint64_t)gridDim.x * (THREADS / LANES);
@@ -104,7 +107,13 @@ __global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackJob job
         float t[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) t[k] = mt::unpack_value(pair[u], (q[u][0] >> (8 * k)) & 255u);
-        if (lane * 4u < at[u].count) *reinterpret_cast<float4 *>(p + lane * 4u) = make_float4(t[0], t[1], t[2], t[3]);
+        if (lane * 4u < at[u].count) {
+          const floatx4 v = {t[0], t[1], t[2], t[3]};
+          if (PAST)
+            __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(p + lane * 4u));
+          else
+            *reinterpret_cast<floatx4 *>(p + lane * 4u) = v;
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -114,18 +123,23 @@ __global__ __launch_bounds__(THREADS) void unpack_kernel(float *out, PackJob job
   }
 }
 
-// calls f with the job, whether a lane's four values are one access, and the width that a group's number needs
+// calls f with the job, how a lane accesses its four values (singly, as one access, as one access past the caches: option
+// "nontemporal"), and the width that a group's number needs
 template <class F>
 void with_job(const PackedView &v, const float *tensor, F &&f) {
   PackJob job{v, (uint64_t)v.w * v.groups, v.n % mt::PACK_GROUP != 0};
   const uint64_t blocks = (job.total + THREADS / LANES * AT_ONCE - 1) / (THREADS / LANES * AT_ONCE);
   const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
-  const bool vec = v.n % 4 == 0 && ((uintptr_t)tensor & 15u) == 0;
-  if (job.rows && job.total > 0xffffffffull) {
-    if (vec) f(job, grid, std::true_type{}, uint64_t{}); else f(job, grid, std::false_type{}, uint64_t{});
-  } else {
-    if (vec) f(job, grid, std::true_type{}, uint32_t{}); else f(job, grid, std::false_type{}, uint32_t{});
-  }
+  const bool vec = v.n % 4 == 0 && ((uintptr_t)tensor & 15u) == 0, past = vec && mt::past_caches((size_t)v.w * v.n * 4);
+  const auto with_index = [&](auto vec_, auto past_) {
+    if (job.rows && job.total > 0xffffffffull) f(job, grid, vec_, past_, uint64_t{}); else f(job, grid, vec_, past_, uint32_t{});
+  };
+  if (past)
+    with_index(std::true_type{}, std::true_type{});
+  else if (vec)
+    with_index(std::true_type{}, std::false_type{});
+  else
+    with_index(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
@@ -150,8 +164,8 @@ int mt_pack(const mt_packed_tensor *out, const mt_tensor *in) {
   if (mt::overlap(in, v)) return mt::fail(MT_E_ARGUMENT, "mt_pack: the packed tensor shares memory with the input");
   mt::note_write(v.q, mt::packed_bytes(v));
   mt::ProfileScope prof("mt_pack");
-  with_job(v, in->p, [&](const PackJob &job, unsigned grid, auto vec, auto index) {
-    pack_kernel<decltype(vec)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(job, in->p);
+  with_job(v, in->p, [&](const PackJob &job, unsigned grid, auto vec, auto past, auto index) {
+    pack_kernel<decltype(vec)::value, decltype(past)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(job, in->p);
   });
   MT_LAUNCH_CHECK("mt_pack");
   return MT_OK;
@@ -166,8 +180,8 @@ int mt_unpack(const mt_tensor *out, const mt_packed_tensor *in) {
   if (mt::overlap(out, v)) return mt::fail(MT_E_ARGUMENT, "mt_unpack: the packed tensor shares memory with the output");
   mt::note_write(out);
   mt::ProfileScope prof("mt_unpack");
-  with_job(v, out->p, [&](const PackJob &job, unsigned grid, auto vec, auto index) {
-    unpack_kernel<decltype(vec)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(out->p, job);
+  with_job(v, out->p, [&](const PackJob &job, unsigned grid, auto vec, auto past, auto index) {
+    unpack_kernel<decltype(vec)::value, decltype(past)::value, decltype(index)><<<grid, THREADS, 0, mt::stream()>>>(out->p, job);
   });
   MT_LAUNCH_CHECK("mt_unpack");
   return MT_OK;

@@ -120,10 +120,26 @@ class Discriminator:
         # keeps it.  step() always runs the whole sequence; a caller that only wants outputs in training mode and the
         # reference's statistics afterwards saves self.stats before and restores them after.
         self.stats = {k: CTensor.from_numpy(host[k] if k in host else v) for k, v in make_statistics().items()}
+        self.g = {}
         self.x, self.labels = CTensor(b, 3, IMAGE, IMAGE), CTensor(b, 1, 1, 1)
+        for i in range(4):
+            for name in ("kernel", "bias", "gamma", "beta"):
+                self.g["%s%d" % (name, i)] = CTensor(*host["%s%d" % (name, i)].shape)
+        self.g["lin_w"], self.g["lin_b"] = CTensor(1, 1, 1, CHANNELS[4] * 16), CTensor(1, 1, 1, 1)
+        self.d_x = CTensor(b, 3, IMAGE, IMAGE)
+        self.logit, self.prob, self.err, self.d_logit = (CTensor(b, 1, 1, 1) for _ in range(4))
+        self.zero_bias = [CTensor.from_numpy(np.zeros((1, CHANNELS[i + 1], 1, 1), np.float32)) for i in range(4)]
+        self.m = {k: CTensor.from_numpy(np.zeros(t.shape, np.float32)) for k, t in self.p.items()}
+        self.v = {k: CTensor.from_numpy(np.zeros(t.shape, np.float32)) for k, t in self.p.items()}
+        self.iteration = 0
+        self._make_activations()
+
+    def _make_activations(self):
+        """The tensors that forward and backward passes leave their values in."""
+        b = self.batch
         self.c, self.bn, self.a, self.xhat, self.ivar = [], [], [], [], []
         self.d_a, self.d_bn, self.d_c = [], [], []
-        self.dk_batch, self.db_batch, self.g = [], [], {}
+        self.dk_batch, self.db_batch = [], []
         self.stat = []
         size = IMAGE
         for i in range(4):
@@ -136,17 +152,8 @@ class Discriminator:
             self.stat.append([CTensor(*s1) for _ in range(4)])      # scratch of the batch-norm backward pass
             self.dk_batch.append(CTensor(b, 1, cout, cin * 16))
             self.db_batch.append(CTensor(b, cout, 1, 1))
-            for name in ("kernel", "bias", "gamma", "beta"):
-                self.g["%s%d" % (name, i)] = CTensor(*host["%s%d" % (name, i)].shape)
-        self.d_x = CTensor(b, 3, IMAGE, IMAGE)
-        self.logit, self.prob, self.err, self.d_logit = (CTensor(b, 1, 1, 1) for _ in range(4))
         self.tmp = [CTensor(*t.shape) for t in self.c]               # elementwise scratch, one per layer size
         self.tmp_dw = CTensor(b, 1, 1, CHANNELS[4] * 16)
-        self.g["lin_w"], self.g["lin_b"] = CTensor(1, 1, 1, CHANNELS[4] * 16), CTensor(1, 1, 1, 1)
-        self.zero_bias = [CTensor.from_numpy(np.zeros((1, CHANNELS[i + 1], 1, 1), np.float32)) for i in range(4)]
-        self.m = {k: CTensor.from_numpy(np.zeros(t.shape, np.float32)) for k, t in self.p.items()}
-        self.v = {k: CTensor.from_numpy(np.zeros(t.shape, np.float32)) for k, t in self.p.items()}
-        self.iteration = 0
 
     def set_batch(self, x, labels):
         self.x.upload(x)
@@ -340,3 +347,74 @@ class Discriminator:
         self.forward(fused)
         self.backward(fused)
         self.update(fused=fused)
+
+    def kept_bytes(self):
+        """Device memory that holds what the forward pass leaves for the backward pass (fused): every layer's input and every
+        batch norm's xhat."""
+        return 4 * sum(t.count for t in [self.x] + self.a + self.xhat)
+
+
+class PackedDiscriminator(Discriminator):
+    """The same training step (its fused form) with what the forward pass leaves for the backward pass kept in 8 bits: the inputs
+    of the convolution and linear layers and the xhat of the batch norms, 1.0625 bytes per value instead of 4.  The fp32 tensors
+    in between are one set of the largest layer's size that all layers use in turn."""
+
+    def _make_activations(self):
+        b, size = self.batch, IMAGE
+        self.shapes, self.ivar, self.kept_a, self.kept_xhat = [], [], [], []
+        for i in range(4):
+            size //= 2
+            self.shapes.append((b, CHANNELS[i + 1], size, size))
+            self.ivar.append(CTensor(1, *self.shapes[i][1:]))
+            self.kept_a.append(mt.CPackedTensor(*self.shapes[i]))
+            self.kept_xhat.append(mt.CPackedTensor(*self.shapes[i]))
+        self.scratch = {k: CTensor(*self.shapes[0]) for k in ("c", "a", "xhat", "d_a", "d_c")}     # the first layer's are the largest
+
+    def _view(self, name, i):
+        t = CTensor.wrap(self.scratch[name].ptr.value, self.shapes[i])
+        t._base = self.scratch[name]
+        return t
+
+    def forward(self, fused=True):
+        if not fused:
+            raise ValueError("activations in 8 bits are a form of the fused step")
+        h, p = self.x, self.p
+        for i in range(4):
+            c, a, xhat = (self._view(k, i) for k in ("c", "a", "xhat"))
+            CTensorConv.ForwardConvolution(c, h, p["kernel%d" % i], 4, 4, CHANNELS[i], CHANNELS[i + 1], p["bias%d" % i], 2, 2, 1, 1)
+            Fused.BatchNormForwardTrain(a, c, p["gamma%d" % i], p["beta%d" % i], xhat, self.ivar[i], new_mean=self.stats["mean%d" % i],
+                                        new_variable=self.stats["variable%d" % i], momentum=MOMENTUM, epsilon=BN_EPSILON, func="leaky_relu")
+            CTensorMath.Pack(self.kept_xhat[i], xhat)
+            CTensorMath.Pack(self.kept_a[i], a)
+            h = a
+        Fused.LinearForward(self.logit, p["lin_w"], h.reinterpret(self.batch, 1, CHANNELS[4] * 16, 1), p["lin_b"])
+        CTensorApplyFunc.ApplySigmoid(self.prob, self.logit)
+        return self.prob
+
+    def backward(self, fused=True):
+        if not fused:
+            raise ValueError("activations in 8 bits are a form of the fused step")
+        b, p, g = self.batch, self.p, self.g
+        Fused.FillMany([g[k] for k in g if not k.startswith("lin")], 0.0)      # the linear layer's are written, not accumulated
+        CTensorMath.Sub(self.err, self.prob, self.labels)
+        CTensorApplyFunc.ApplyDifferentialSigmoid(self.d_logit, self.logit)
+        CTensorMath.TensorItemProduction(self.d_logit, self.err, self.d_logit)
+        delta = self._view("d_a", 3)
+        CTensorMath.TransponseMul(delta.reinterpret(b, 1, CHANNELS[4] * 16, 1), p["lin_w"], self.d_logit)
+        Fused.LinearBackwardWeightsSum(g["lin_w"], g["lin_b"], self.kept_a[3], self.d_logit, accumulate=False)
+        for i in (3, 2, 1, 0):
+            xhat, d_c = self._view("xhat", i), self._view("d_c", i)
+            CTensorMath.Unpack(xhat, self.kept_xhat[i])
+            Fused.BatchNormBackward(d_c, g["gamma%d" % i], g["beta%d" % i], delta, p["gamma%d" % i], xhat, self.ivar[i], beta=p["beta%d" % i], func="leaky_relu")
+            inp, prev = (self._view("a", i - 1), self._view("d_a", i - 1)) if i else (self.x, self.d_x)
+            if i:
+                CTensorMath.Unpack(inp, self.kept_a[i - 1])
+            CTensorConv.BackwardConvolution(prev, d_c, p["kernel%d" % i], 4, 4, CHANNELS[i], CHANNELS[i + 1], self.zero_bias[i], 2, 2, 1, 1)
+            Fused.ConvolutionBackwardWeightsSum(g["kernel%d" % i], 4, 4, CHANNELS[i], CHANNELS[i + 1], g["bias%d" % i], inp, d_c, 2, 2, 1, 1)
+            delta = prev
+
+    def step(self, fused=True):
+        super().step(fused)
+
+    def kept_bytes(self):
+        return 4 * self.x.count + sum(t.nbytes for t in self.kept_a + self.kept_xhat)

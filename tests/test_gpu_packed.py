@@ -281,3 +281,42 @@ def test_another_stream(mt):
         mt.set_stream(None)
         hip.hipStreamDestroy(stream)
     assert all(np.array_equal(got[k], want[k]) for k in RESULTS)
+
+
+@pytest.mark.parametrize("batch", [4, 16])
+def test_a_discriminator_with_activations_in_8_bits(mt, batch):
+    """The discriminator's training step with its activations kept in 8 bits: the gradients of the ordinary step on activations that
+    went through 8 bits, bit for bit but for the linear layer's product; and near those of the fp32 step."""
+    import discriminator as D
+    params = D.make_parameters()
+    x, labels = D.make_batch(batch)
+    plain, packed = D.Discriminator(batch, params), D.PackedDiscriminator(batch, params)
+    for net in (plain, packed):
+        net.set_batch(x, labels)
+        net.forward(True)
+    assert np.array_equal(plain.prob.numpy(), packed.prob.numpy())
+    plain.backward(True)
+    fp32 = {k: t.numpy().astype(np.float64) for k, t in plain.g.items()}
+    for t in plain.a + plain.xhat:
+        kept = mt.CPackedTensor(*t.shape)
+        mt.CTensorMath.Pack(kept, t)
+        mt.CTensorMath.Unpack(t, kept)
+    plain.backward(True)
+    packed.backward()
+    for k in plain.g:
+        a, b = plain.g[k].numpy().astype(np.float64), packed.g[k].numpy().astype(np.float64)
+        # fp32 sums of `batch` products in two orders: 2 * batch roundings of sums that are at most batch times their terms
+        assert np.array_equal(a, b) if not k.startswith("lin") else np.linalg.norm(a - b) <= 2 * batch * batch * po.U * np.linalg.norm(a), k
+    assert np.array_equal(plain.d_x.numpy(), packed.d_x.numpy())
+    # xhat within 1/255 of a range of seven deviations turns the sign of gamma*xhat+beta, and so the slope of the leaky ReLU from 0.1 to
+    # 1, for 0.4 * 2 * 7/255/4 = 0.5 % of the values of a layer: 0.9 / 0.7 * sqrt(0.005) = 9 % of a delta's norm per layer, 18 % over four
+    for k, want in fp32.items():
+        got = packed.g[k].numpy().astype(np.float64)
+        if not k.startswith("bias"):                # in front of a batch norm a bias has no gradient but rounding
+            assert np.linalg.norm(got - want) <= 0.25 * np.linalg.norm(want), k
+    # all but the images: 1 + 8/128 bytes per value instead of 4 (every sample is a whole number of groups)
+    images = 4 * plain.x.count
+    assert 64 * (packed.kept_bytes() - images) == 17 * (plain.kept_bytes() - images)
+    packed.update(fused=True)
+    packed.step()
+    assert all(np.isfinite(t.numpy()).all() for t in packed.p.values())

@@ -172,7 +172,7 @@ struct Forward {
   const float *in, *gamma, *beta;
   float *mean, *ivar;  // null: not wanted
   PackedView packed;
-  uint32_t rows, N, per_sample;
+  uint32_t first_row, rows, N, per_sample;  // first_row: of this launch
   float eps;
   int func;
 };
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
   __shared__ float part[2][L / 64 + 1];
-  const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
+  const uint32_t want = a.first_row + blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
   const bool mine = want < a.rows;
   float x[E];
   S::template load<ACCESS>(x, a.in + (size_t)row * a.N, a.N);
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 // from delta and x: they need no sum over a row.  That reads both a second time, from the caches, where the kernel above writes and
 // joins partial sums: 256 rows of 4096 10.7 -> 5.2 us, 33 of 1001 7.0 -> 4.9; 8192 of 2048 would lose (36 us against 50).
 template <int L, int E, int ACCESS, bool FUNC, class Rows>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t error_blocks) {
+__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t first_row, uint32_t error_blocks) {
   constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, VEC>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
     return;
   }
   __shared__ float part[2][L / 64 + 1];
-  const uint32_t want = blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
+  const uint32_t want = first_row + blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
   const float mean = a.mean[row], ivar = a.ivar[row];
   const auto in = rows.row(row);
   typename Rows::template Raw<VEC> raw[S::STEPS];
@@ -773,24 +773,33 @@ bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { 
 // pieces, 2000 x 16383 185 against 129
 constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384, BACKWARD_ROW_TIGHT = 8192;
 
+// blocks of one launch, at most: a grid has fewer than 2^32 threads
+constexpr uint32_t MOST_BLOCKS = 1u << 21;
+
 template <int L, int E>
-void forward_rows(const Forward &a, int access, bool pack) {
-  const unsigned grid = cdiv(a.rows, L < 256 ? 256 / L : 1), threads = L < 256 ? 256 : L;
-  if constexpr (L >= 64) {
-    if (pack) {
-      if (access == FOUR_PAST)
-        ln_forward_kernel<L, E, FOUR_PAST, true><<<grid, threads, 0, mt::stream()>>>(a);
-      else
-        ln_forward_kernel<L, E, FOUR, true><<<grid, threads, 0, mt::stream()>>>(a);
-      return;
-    }
+void forward_rows(Forward a, int access, bool pack) {
+  constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
+  for (;;) {
+    const uint32_t left = a.rows - a.first_row, grid = cdiv(left, PER_BLOCK) < MOST_BLOCKS ? cdiv(left, PER_BLOCK) : MOST_BLOCKS;
+    const auto go = [&](auto acc) {
+      constexpr int ACCESS = decltype(acc)::value;
+      if constexpr (L >= 64 && ACCESS != ONE) {
+        if (pack) {
+          ln_forward_kernel<L, E, ACCESS, true><<<grid, BLOCK, 0, mt::stream()>>>(a);
+          return;
+        }
+      }
+      ln_forward_kernel<L, E, ACCESS, false><<<grid, BLOCK, 0, mt::stream()>>>(a);
+    };
+    if (access == FOUR_PAST)
+      go(std::integral_constant<int, FOUR_PAST>{});
+    else if (access == FOUR)
+      go(std::integral_constant<int, FOUR>{});
+    else
+      go(std::integral_constant<int, ONE>{});
+    if (left <= grid * PER_BLOCK) return;
+    a.first_row += grid * PER_BLOCK;
   }
-  if (access == FOUR_PAST)
-    ln_forward_kernel<L, E, FOUR_PAST, false><<<grid, threads, 0, mt::stream()>>>(a);
-  else if (access == FOUR)
-    ln_forward_kernel<L, E, FOUR, false><<<grid, threads, 0, mt::stream()>>>(a);
-  else
-    ln_forward_kernel<L, E, ONE, false><<<grid, threads, 0, mt::stream()>>>(a);
 }
 
 // calls f with the threads per row and the values per thread that hold a row of N values
@@ -855,16 +864,19 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         const uint32_t per_block = L < 256 ? 256 / L : 1, threads = L < 256 ? 256 : L;
         if (beside) {
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
-          const auto go = [&](uint32_t grid, uint32_t first_param_block) {
+          const auto go = [&](uint32_t first_row, uint32_t grid, uint32_t first_param_block) {
             with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
-              ln_backward_few_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_param_block);
+              ln_backward_few_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_row, first_param_block);
             });
           };
-          if (a.error == a.delta && params) {  // written in place: the sums before the error
-            go(param_blocks, 0);
-            go(error_blocks, error_blocks);
+          if (params && a.error != a.delta) {
+            go(0, error_blocks + param_blocks, error_blocks);
           } else {
-            go(error_blocks + param_blocks, error_blocks);
+            if (params) go(0, param_blocks, 0);  // written in place: the sums before the error
+            for (uint32_t b = 0; b < error_blocks; b += MOST_BLOCKS) {
+              const uint32_t grid = error_blocks - b < MOST_BLOCKS ? error_blocks - b : MOST_BLOCKS;
+              go(b * per_block, grid, grid);
+            }
           }
           return (int)MT_OK;
         }
@@ -895,7 +907,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     uint32_t per_group = cdiv(g.rows, groups);
     if (per_group > GROUP_ROWS) per_group = GROUP_ROWS;
     groups = cdiv(g.rows, per_group);
-    if ((uint64_t)g.rows * pieces > 0x7fffffffull || (uint64_t)groups * strips > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
+    if ((uint64_t)g.rows * pieces >= (1u << 24) || (uint64_t)groups * strips >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
     const size_t sums = 2 * (size_t)g.rows * pieces;
     float *ws = nullptr;
     int rc = ln_workspace(sums + (params && groups > 1 ? 2 * (size_t)groups * g.N : 0), &ws);
@@ -1005,7 +1017,7 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
       MT_LAUNCH_CHECK(name);
     } else {
       const uint32_t pieces = cdiv(g.N, PIECE);
-      if ((uint64_t)g.rows * pieces > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
+      if ((uint64_t)g.rows * pieces >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many elements for one launch", name);
       float *ws = nullptr;
       if ((rc = ln_workspace(2 * (size_t)g.rows * pieces, &ws))) return rc;
       float2 *stats = reinterpret_cast<float2 *>(ws);

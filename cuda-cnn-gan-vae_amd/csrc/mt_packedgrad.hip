@@ -388,6 +388,7 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   if (dbias && (dbias->w != 1 || dbias->z != 1 || dbias->x != 1 || dbias->y != out)) return mt::fail(MT_E_SHAPE, "%s: dbias must be [1,1,Out,1]", name);
   // the rows of a step are addressed with 32-bit offsets
   if (v.n >= (1u << 24) || out >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: 2^24 features or more are not supported", name);
+  if (v.w >= 0x7fff0000u) return mt::fail(MT_E_UNAVAILABLE, "%s: nearly 2^31 samples or more are not supported", name);
   const uint32_t Out = (uint32_t)out;
   if (Out == 0) return MT_OK;
   for (auto t : {dweight, dbias})
@@ -429,7 +430,7 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
     a.dbias = dbias ? dbias->p : nullptr;
   }
   const size_t grid = tiles * a.split;
-  if (grid > 0x7fffffffull) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);
+  if (grid >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);  // a grid has fewer than 2^32 threads
   if (wide)
     packed_wgrad_kernel<2, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
   else if (pair)

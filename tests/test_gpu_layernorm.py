@@ -329,3 +329,28 @@ def test_more_than_2_31_elements(mt):
     assert np.array_equal(view(out).numpy(), kept)
     for t in (big, out, dl, pk, mean, ivar):
         t.free()
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_more_rows_than_one_launch_takes(mt, n):
+    """Rows of one and two values, more than 2^26 of them: 32 rows per block, at most 2^21 blocks per launch."""
+    rows, tail = (1 << 26) + 77, 40
+    x, gamma, beta, delta = inputs(4, (tail, 1, n, 1), (1, 1, n, 1))
+    big, out = mt.CTensor(rows, 1, n, 1), mt.CTensor(rows, 1, n, 1)
+    mean, ivar = mt.CTensor(rows, 1, 1, 1), mt.CTensor(rows, 1, 1, 1)
+    mt.CTensorMath.Fill(big, 0.25)
+    mt.CTensorMath.Fill(out, 9.0)
+    view = lambda t, k=n: mt.CTensor.wrap(t.ptr.value + (rows - tail) * k * 4, (tail, 1, k, 1))
+    view(big).upload(x)
+    tg, tb = up(mt, gamma), up(mt, beta)
+    mt.Fused.LayerNormForward(out, big, tg, tb, mean, ivar)
+    want = run_forward(mt, x, gamma, beta)
+    assert np.array_equal(view(out).numpy(), want[0]) and np.array_equal(view(mean, 1).numpy(), want[1]) and np.array_equal(view(ivar, 1).numpy(), want[2])
+    middle = mt.CTensor.wrap(out.ptr.value + ((1 << 26) - 8) * n * 4, (16, 1, n, 1)).numpy()      # on both sides of the first launch's end
+    assert np.array_equal(middle, np.broadcast_to(beta, middle.shape))                        # a constant row: xhat is 0
+    view(out).upload(delta)
+    mt.Fused.LayerNormBackward(out, None, None, out, tg, big, mean, ivar)
+    small = run_backward(mt, delta, x, gamma, beta, want[1], want[2])
+    assert np.array_equal(view(out).numpy(), small["error"])
+    for t in (big, out, mean, ivar):
+        t.free()

@@ -36,23 +36,34 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
 
 // ---- the functions of the function layer that the kernels hold: the values of f_sigmoid_fast and f_tangence_fast, with a reciprocal
 // that is not a division (two thirds of the instructions; 32 rows of 147456 with sigmoid 12.8 -> 11.8 us) ---------------------------
-__device__ __forceinline__ float sigmoid(float v) {
+// (`e` the exponential, `r` the reciprocal of 1 + e: the derivatives are (1 - f) * f = e * r * r and 1 - f * f = 4 * e * r * r, without the
+// difference of two neighbouring numbers)
+struct Exponential {
+  float e, r;
+};
+__device__ __forceinline__ Exponential exponential(float v) {
+  Exponential t;
+  t.e = __expf(v);
+  t.r = mt::reciprocal(1.f + t.e);
+  return t;
+}
+__device__ __forceinline__ Exponential for_sigmoid(float v) {
   if (v > 30.f) v = 29.99999f;
   if (v < -30.f) v = -29.99999f;
-  return mt::reciprocal(1.f + __expf(-v));
+  return exponential(-v);
 }
-__device__ __forceinline__ float tangence(float v) {
+__device__ __forceinline__ Exponential for_tangence(float v) {
   if (v > 30.f) v = 30.f;  // 1 from there on; an infinite exponential has no reciprocal here
-  return 1.f - 2.f * mt::reciprocal(__expf(2.f * v) + 1.f);
+  return exponential(2.f * v);
 }
 template <int N>
 __device__ __forceinline__ void apply(int func, float *v) {
   if (func == MT_F_SIGMOID) {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = sigmoid(v[i]);
+    for (int i = 0; i < N; i++) v[i] = for_sigmoid(v[i]).r;
   } else if (func == MT_F_TANGENCE) {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = tangence(v[i]);
+    for (int i = 0; i < N; i++) v[i] = 1.f - 2.f * for_tangence(v[i]).r;
   } else {
     mt::apply_func_cheap_many<N>(func, v);
   }
@@ -313,27 +324,27 @@ __device__ __forceinline__ void fronts(int func, float *g, const float *gamma, c
   } else if (func == MT_F_SIGMOID) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const float f = sigmoid(gamma[i] * xhat[i] + beta[i]);
-      g[i] *= (1.f - f) * f;
+      const Exponential t = for_sigmoid(gamma[i] * xhat[i] + beta[i]);
+      g[i] *= t.e * t.r * t.r;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const float f = tangence(gamma[i] * xhat[i] + beta[i]);
-      g[i] *= 1.f - f * f;
+      const Exponential t = for_tangence(gamma[i] * xhat[i] + beta[i]);
+      g[i] *= 4.f * (t.e * t.r) * t.r;
     }
   }
 }
 
-// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g): 64 columns per SLICES wavefronts, which take every
-// SLICES-th row with eight loads in flight, joined in a fixed order.  Many parts: sixteen wavefronts (four took 7.4 us for 512 rows of
-// 2000, waiting for one batch of loads after the other; sixteen take 3).  Few parts of long rows: one (sixteen took 14 us for
-// 8 rows of 147456).
-constexpr uint32_t JOIN_MANY = 16;
+// the sums of `parts` rows of partial sums [2][parts][N] (of g * xhat, of g), joined in a fixed order.  Many parts: 32 columns per
+// block, whose 32 slices take every 32nd row with eight loads under way (4 slices of 64 columns took 7.4 us for 512 rows of 2000, waiting
+// for one batch of loads after the other; 16 of 64 take 4.8, 32 of 32 another 0.6 to 0.9 less).  Few parts of long rows: a
+// thread per column (16 slices took 14 us for 8 rows of 147456).
+constexpr uint32_t JOIN_MANY = 32, JOIN_COLUMNS = 32;
 template <int SLICES>
-__global__ __launch_bounds__(SLICES == 1 ? THREADS : 64 * SLICES) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N,
+__global__ __launch_bounds__(SLICES == 1 ? THREADS : JOIN_COLUMNS * SLICES) void ln_join_kernel(float *dgamma, float *dbeta, const float *partial, uint32_t parts, uint32_t N,
                                                                                      bool accumulate) {
-  constexpr uint32_t COLUMNS = SLICES == 1 ? THREADS : 64;
+  constexpr uint32_t COLUMNS = SLICES == 1 ? THREADS : JOIN_COLUMNS;
   __shared__ float sums[SLICES][COLUMNS];
   const uint32_t i = blockIdx.x * COLUMNS + threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS;
   float *out = blockIdx.y == 0 ? dgamma : dbeta;
@@ -630,87 +641,99 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
   s2 = row_sum<THREADS>(s2, part[1]);
   if (threadIdx.x == 0) sums[blockIdx.x] = make_float2(s1, s2);
 }
-// ... then blocks of 256 * WIDTH columns that walk over a group of rows: the error, and their columns' share of dgamma and dbeta
-constexpr uint32_t GROUP_ROWS = 64;  // rows of a group, at most
+// ... then blocks of 64 * WIDTH columns whose four wavefronts take every fourth row of a group: the error, and their columns' share of
+// dgamma and dbeta, added in LDS.  Where the columns alone make enough blocks there is one group, and no sums are left to join
+// (32 rows of 196608 with tangence 24.8 us; 28.8 with four groups of rows that each wrote their sums for a third launch).
+constexpr uint32_t GROUP_ROWS = 256;  // rows of a group, at most
 template <int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a, Rows rows, const float2 *sums, uint32_t pieces, uint32_t groups, uint32_t per_group,
                                                                      float *partial) {
   constexpr bool VEC = ACCESS != ONE;
-  constexpr int W = VEC ? 4 : 1;
+  constexpr uint32_t W = VEC ? 4 : 1, SLICES = THREADS / 64, AT_ONCE = 4;
   __shared__ float4 terms[GROUP_ROWS];  // of each row: mean, ivar, sum(u) / N, sum(u * xhat) / N
-  const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * THREADS + threadIdx.x) * W, at = min(column, a.N - W);
-  const uint32_t first = group * per_group, count = min(per_group, a.rows - first), lane = threadIdx.x % 64;
-  for (uint32_t k = threadIdx.x / 64; k < count; k += THREADS / 64) {
-    const float2 *p = sums + (size_t)(first + k) * pieces;
-    float s1 = 0.f, s2 = 0.f;
-    for (uint32_t i = lane; i < pieces; i += 64) {
-      s1 += p[i].x;
-      s2 += p[i].y;
-    }
-    s1 = mt::over_lanes<mt::Sum, 64>(s1) / (float)a.N;
-    s2 = mt::over_lanes<mt::Sum, 64>(s2) / (float)a.N;
-    if (lane == 0) terms[k] = make_float4(a.mean[first + k], a.ivar[first + k], s1, s2);
-  }
-  // gamma and beta repeated for the rows that are taken at once
-  constexpr uint32_t AT_ONCE = 4;
-  float gamma[AT_ONCE][W], beta[AT_ONCE][W], dg[W] = {}, db[W] = {};
-#pragma unroll
-  for (uint32_t u = 0; u < AT_ONCE; u++) {
-    load_step<VEC ? FOUR : ONE>(gamma[u], a.gamma, at);
-    if (FUNC) load_step<VEC ? FOUR : ONE>(beta[u], a.beta, at);
-  }
-  __syncthreads();
-  // four rows at a time, loaded before the first of them is stored (the error may be written over delta: each thread reads and
-  // writes its own columns)
-  for (uint32_t k0 = 0; k0 < count; k0 += AT_ONCE) {
-    typename Rows::template Raw<VEC> raw[AT_ONCE];
-    float x[AT_ONCE][W], g[AT_ONCE][W];
+  __shared__ float shares[2][SLICES][W][64];
+  const uint32_t lane = threadIdx.x % 64, slice = threadIdx.x / 64;
+  const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * 64 + lane) * W, at = min(column, a.N - W);
+  const uint32_t first = group * per_group, count = min(per_group, a.rows - first);
+  // four rows at a time, the next four loaded before the first of them is stored (the error may be written over delta: each row of a
+  // column is read and written by one thread)
+  typename Rows::template Raw<VEC> raw[AT_ONCE], raw_n[AT_ONCE];
+  float g[AT_ONCE][W], g_n[AT_ONCE][W];
+  const auto load = [&](uint32_t k0, typename Rows::template Raw<VEC> *r, float (*d)[W]) {
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
-      const uint32_t row = first + min(k0 + u, count - 1);
-      load_step<ACCESS>(g[u], a.delta + (size_t)row * a.N, at);
-      rows.row(row).template load<ACCESS>(raw[u], at);
+      const uint32_t row = first + min(k0 + u * SLICES, count - 1);
+      load_step<ACCESS>(d[u], a.delta + (size_t)row * a.N, at);
+      rows.row(row).template load<ACCESS>(r[u], at);
     }
+  };
+  load(slice, raw, g);
+  float gamma[W], beta[W], dg[W] = {}, db[W] = {};
+  load_step<VEC ? FOUR : ONE>(gamma, a.gamma, at);
+  if (FUNC) load_step<VEC ? FOUR : ONE>(beta, a.beta, at);
+  // eight lanes per row, eight loads each under way
+  for (uint32_t k = threadIdx.x / 8; k < count; k += THREADS / 8) {
+    const float2 *p = sums + (size_t)(first + k) * pieces;
+    float s1 = 0.f, s2 = 0.f;
+    for (uint32_t i = threadIdx.x % 8; i < pieces; i += 64) {
+      float2 t[8];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) t[u] = p[min(i + 8 * u, pieces - 1)];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) {
+        s1 += i + 8 * u < pieces ? t[u].x : 0.f;
+        s2 += i + 8 * u < pieces ? t[u].y : 0.f;
+      }
+    }
+    s1 = mt::over_lanes<mt::Sum, 8>(s1) / (float)a.N;
+    s2 = mt::over_lanes<mt::Sum, 8>(s2) / (float)a.N;
+    if (threadIdx.x % 8 == 0) terms[k] = make_float4(a.mean[first + k], a.ivar[first + k], s1, s2);
+  }
+  __syncthreads();
+  for (uint32_t k0 = slice; k0 < count; k0 += AT_ONCE * SLICES) {
+    if (k0 + AT_ONCE * SLICES < count) load(k0 + AT_ONCE * SLICES, raw_n, g_n);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
-      raw[u].values(x[u]);
-      const float4 c = terms[min(k0 + u, count - 1)];
+      const uint32_t k = k0 + u * SLICES;
+      if (k >= count) break;
+      const float4 c = terms[k];
+      float x[W], t[W];
+      raw[u].values(x);
 #pragma unroll
-      for (int e = 0; e < W; e++) x[u][e] = (x[u][e] - c.x) * c.y;
+      for (uint32_t e = 0; e < W; e++) x[e] = (x[e] - c.x) * c.y;
+      if constexpr (FUNC) fronts<W>(a.func, g[u], gamma, x, beta);
+#pragma unroll
+      for (uint32_t e = 0; e < W; e++) {
+        dg[e] += g[u][e] * x[e];
+        db[e] += g[u][e];
+        t[e] = c.y * ((g[u][e] * gamma[e] - c.z) - x[e] * c.w);
+      }
+      if (column < a.N) store_step<ACCESS>(a.error + (size_t)(first + k) * a.N + column, t);
     }
-    if constexpr (FUNC) fronts<AT_ONCE * W>(a.func, g[0], gamma[0], x[0], beta[0]);
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
-      if (k0 + u >= count) break;
-      const float4 c = terms[k0 + u];
-      float t[W];
+      raw[u] = raw_n[u];
 #pragma unroll
-      for (int e = 0; e < W; e++) {
-        dg[e] += g[u][e] * x[u][e];
-        db[e] += g[u][e];
-        t[e] = c.y * ((g[u][e] * gamma[u][e] - c.z) - x[u][e] * c.w);
-      }
-      if (column < a.N) {
-        store_step<ACCESS>(a.error + (size_t)(first + k0 + u) * a.N + column, t);
-      }
+      for (uint32_t e = 0; e < W; e++) g[u][e] = g_n[u][e];
     }
   }
-  if (column >= a.N) return;
-  if (groups > 1) {
-    float *pg = partial + (size_t)group * a.N + column, *pb = partial + ((size_t)groups + group) * a.N + column;
-    if (a.dgamma || a.dbeta)
 #pragma unroll
-      for (int e = 0; e < W; e++) {
-        pg[e] = dg[e];
-        pb[e] = db[e];
-      }
-    return;
+  for (uint32_t e = 0; e < W; e++) {
+    shares[0][slice][e][lane] = dg[e];
+    shares[1][slice][e][lane] = db[e];
   }
+  __syncthreads();
+  if (slice > 1 || column >= a.N) return;
+  float *out = slice == 0 ? a.dgamma : a.dbeta;
+  if (out == nullptr) return;
+  if (groups > 1) out = partial + ((size_t)slice * groups + group) * a.N;
 #pragma unroll
-  for (int e = 0; e < W; e++) {
-    if (a.dgamma) a.dgamma[column + e] = a.accumulate ? a.dgamma[column + e] + dg[e] : dg[e];
-    if (a.dbeta) a.dbeta[column + e] = a.accumulate ? a.dbeta[column + e] + db[e] : db[e];
+  for (uint32_t e = 0; e < W; e++) {
+    float s = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < SLICES; k++) s += shares[slice][k][e][lane];
+    out[column + e] = a.accumulate && groups == 1 ? out[column + e] + s : s;
   }
 }
 
@@ -899,11 +922,12 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     if (rc) return rc;
     MT_LAUNCH_CHECK(name);
   } else {
-    const uint32_t pieces = cdiv(g.N, PIECE), strips = cdiv(g.N, THREADS * (vec ? 4 : 1));
-    // enough blocks to keep the memory busy, but groups of at least 8 rows: every group writes and joins 16 bytes per column where a
+    const uint32_t pieces = cdiv(g.N, PIECE), strips = cdiv(g.N, 64 * (vec ? 4 : 1));
+    // enough blocks to keep the memory busy, but groups of at least 16 rows: every group writes and joins 16 bytes per column where a
     // row moves 20
-    uint32_t groups = cdiv(1024, strips);
-    if (groups > cdiv(g.rows, 8)) groups = cdiv(g.rows, 8);
+    const uint32_t blocks = vec ? 768 : 2048;  // that the compute units hold at once
+    uint32_t groups = strips < blocks / 2 ? blocks / strips : 1;
+    if (groups > cdiv(g.rows, 16)) groups = cdiv(g.rows, 16);
     uint32_t per_group = cdiv(g.rows, groups);
     if (per_group > GROUP_ROWS) per_group = GROUP_ROWS;
     groups = cdiv(g.rows, per_group);
@@ -924,8 +948,8 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     MT_LAUNCH_CHECK(name);
   }
   if (params && parts) {
-    if (parts > JOIN_MANY)
-      ln_join_kernel<JOIN_MANY><<<dim3(cdiv(g.N, 64), 2), 64 * JOIN_MANY, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
+    if (parts > 16)
+      ln_join_kernel<JOIN_MANY><<<dim3(cdiv(g.N, JOIN_COLUMNS), 2), JOIN_COLUMNS * JOIN_MANY, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
     else
       ln_join_kernel<1><<<dim3(cdiv(g.N, THREADS), 2), THREADS, 0, mt::stream()>>>(a.dgamma, a.dbeta, partial, parts, g.N, a.accumulate);
     MT_LAUNCH_CHECK(name);

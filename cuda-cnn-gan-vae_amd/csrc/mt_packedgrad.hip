@@ -4,7 +4,8 @@
 //                 = sum_b (delta * step)[b][o] * (q[b][i] - 128)  +  sum_b delta[b][o] * (low + 128 * step)[b][g]
 //
 // q - 128 is a whole number of 8 bits: exact in bf16.  delta * step, one fp32 product, is the exact sum of three bf16 numbers:
-// its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder exact).  Three bf16
+// its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder exact; products below
+// 2^-110 lose the bits that no normal bf16 number holds).  Three bf16
 // matrix instructions therefore multiply what one fp32 product would, into fp32 accumulators, at a third of the bf16
 // rate (some 800 TFLOP/s) where the fp32 matrix instructions reach 157.  The second sum is one fp32 multiply-add per element of
 // delta on the way.
@@ -358,6 +359,7 @@ Plan choose(uint32_t Out, uint32_t groups, uint32_t steps, size_t n) {
     const double fixed = kind == 0 ? 5.0 : kind == 1 ? 6.0 : 6.5, one = kind == 0 ? 1.75 : kind == 1 ? 3.0 : 2.8, two = kind == 0 ? 3.25 : kind == 1 ? 6.0 : 5.7;
     const size_t tiles = (size_t)cdiv(Out, rows) * groups;
     for (uint32_t split = 1; split <= 128 && split <= steps; split += split < 4 ? 1 : split / 2) {
+      if (split > 1 && n >= (1u << 29)) break;  // a join is one launch of fewer than 2^32 threads
       const size_t blocks = tiles * split;
       const size_t rest = blocks % 512;
       const double turn = blocks / 512 * two + (rest > 256 ? two : rest > 0 ? one : 0.0);
@@ -430,7 +432,7 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
     a.dbias = dbias ? dbias->p : nullptr;
   }
   const size_t grid = tiles * a.split;
-  if (grid >= (1u << 24)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);  // a grid has fewer than 2^32 threads
+  if (grid >= (1u << 23)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);  // a grid has fewer than 2^32 threads
   if (wide)
     packed_wgrad_kernel<2, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
   else if (pair)

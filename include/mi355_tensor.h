@@ -399,8 +399,10 @@ int mt_convolution_backward_weights_sum(const mt_tensor *dkernel, int32_t dkerne
  *   mean = sum(x)/N, ivar = 1/sqrt(sum((x-mean)^2)/N + epsilon), xhat = (x-mean)*ivar, output = func(gamma*xhat + beta).
  * mean and ivar hold one value per row: the input's sizes with 1 in place of those that the row spans.  Sums are fp32, taken in
  * an order that depends on the sizes and on whether the tensors are 16-byte aligned: the same call gives the same bits.
- * A NaN or an infinity in a row makes that row NaN (and the parameter gradients it adds to).  At most 2^31 - 1 rows,
- * of at most 2^31 - 17 values, and 2^36 values in all where the rows are longer than 16384.
+ * A NaN or an infinity in a row makes that row of xhat NaN, and with it the row's error and the dgamma it adds to (what func
+ * makes of a NaN is its own: MT_F_RELU makes it 0).  Values whose squared deviations overflow (1.8e19 from their mean) have an
+ * ivar of 0.  At most 2^31 - 1 rows, of at most 2^31 - 17 values, and fewer than 2^36 values in all where the rows are longer
+ * than 8192.
  * No result may share memory with another tensor, but for the two cases named below.
  *
  * mt_layernorm_forward_func: mean and ivar (NULL to skip) are what the backward pass needs.  output may be the same tensor as
@@ -439,7 +441,8 @@ int mt_unpack(const mt_tensor *output, const mt_packed_tensor *input);          
  * dweight [1,1,Out,In] (+)= sum over the batch of delta (x) value(input), dbias [1,1,Out,1] (NULL to skip) (+)= sum of delta;
  * input [B,...] of In values per sample, delta [B,...] of Out values.  accumulate: 1 adds to what the gradients hold, 0 overwrites.
  * The products are those of the fp32 numbers delta and step with the whole numbers q, summed in fp32; a gradient's bits depend
- * on the sizes only.  A delta that is not a finite number makes its row of dweight NaN.  Fewer than 2^24 features on either side. */
+ * on the sizes only.  A delta that is not a finite number, or whose product with a step is none, makes its row of dweight NaN in
+ * the columns of that group.  Fewer than 2^24 features on either side. */
 int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_tensor *dbias, const mt_packed_tensor *input, const mt_tensor *delta, int accumulate);
 
 /* TrainingResetDeltaWeight of every layer of a network (netlayer/cnetlayerconvolution.cu.h:522-526 and the same

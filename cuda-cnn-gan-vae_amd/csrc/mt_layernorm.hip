@@ -117,6 +117,7 @@ struct Share {
 // ---- where a row's input comes from in the backward pass: the fp32 tensor, or the 8 bits the forward pass kept.  Loading and
 // decoding are two steps, so that all loads of a row are under way before the first is waited for ------------------------------
 struct RowsF32 {
+  static constexpr int BYTES = 4;  // of a value, about
   const float *p;
   uint32_t N;
   template <bool VEC>
@@ -135,6 +136,7 @@ struct RowsF32 {
   __device__ __forceinline__ Row row(uint32_t r) const { return Row{p + (size_t)r * N}; }
 };
 struct RowsPacked {
+  static constexpr int BYTES = 1;
   PackedView v;
   uint32_t N, per_sample;  // rows of one sample
   template <bool VEC>
@@ -912,7 +914,8 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
   }
   const bool params = dgamma || dbeta;
   const bool vec = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
-  const int access = !vec ? ONE : mt::past_caches(mt::count(delta) * 4) ? FOUR_PAST : FOUR;
+  // (half of what the pass moves stands for the size of a tensor that is read and written: 4096 x 6144 62.6 -> 58.2 us)
+  const int access = !vec ? ONE : mt::past_caches(mt::count(delta) * (8 + Rows::BYTES) / 2) ? FOUR_PAST : FOUR;
   // few rows: the parameter gradients beside the error instead of partial sums and their join
   const bool few = g.rows <= 512;
   uint32_t parts = 0;

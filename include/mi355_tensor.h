@@ -162,8 +162,8 @@ int mt_timer_destroy(void *timer);
  *                    2 (default) products per input pixel on the 16x16x4 matrix instruction where the shape allows /
  *                    1 the 4x4x1 matrix instruction where the shape allows / 0 the vector ALUs
  *   "image_strip"    rows per strip of the image layer's product kernel on images of 64 columns (0, default: 8 or 4)
- *   "nontemporal"    2 (default) the re-sampling, pooling and large-batch batch-norm kernels read and write tensors of 128 MiB
- *                    and more past the caches (each element is touched once) / 1 always / 0 never
+ *   "nontemporal"    2 (default) the re-sampling, pooling, large-batch batch-norm, layer-norm and 8-bit packing kernels read and
+ *                    write tensors of 128 MiB and more past the caches (each element is touched once) / 1 always / 0 never
  *   "staged_uploads" 1 (default) mt_copy_h2d of at most 64 KiB copies the caller's buffer into a pinned slot at once and queues
  *                    the copy to the device behind the work already queued, without waiting for it / 0 every upload waits
  *   "pool"           1 (default) mt_free keeps blocks for the next mt_malloc of the same size (stream-ordered reuse, no

@@ -122,6 +122,52 @@ def test_geometries(mt, shape, pshape, shift, func):
             within(got, back, key)
 
 
+@pytest.mark.parametrize("rows,n,func", [(600, 8196, "tangence"), (257, 16388, None), (530, 8195, "sigmoid"), (17, 16385, None), (300, 20000, "relu"), (16, 49152, None),
+                                         (33, 49156, "tangence"), (520, 17001, None)])
+def test_many_long_rows(mt, rows, n, func):
+    """Sums over rows that are cut into pieces: several groups of rows, groups of every size, error beside and over delta."""
+    x, gamma, beta, delta = inputs(rows + n, (rows, 1, n, 1), (1, 1, n, 1))
+    out, mean, ivar, pk = run_forward(mt, x, gamma, beta, func, packed=True)
+    within(out, po.forward(x, gamma, beta, 1e-6, func), "out")
+    for source, v in ((x, x), (pk, po.through_8_bits(x))):
+        back = po.backward(delta, v, gamma, beta, mean, ivar, func)
+        a, b = run_backward(mt, delta, source, gamma, beta, mean, ivar, func), run_backward(mt, delta, source, gamma, beta, mean, ivar, func, inplace=True)
+        for key, got in a.items():
+            within(got, back, key)
+            assert np.array_equal(got, b[key])
+
+
+@pytest.mark.parametrize("rows,n", [(5, 24), (700, 24), (600, 128), (9, 1024), (600, 1024), (5, 4096), (513, 4096), (7, 8192), (3, 16384), (600, 8192), (3, 32768), (20, 40000)])
+@pytest.mark.parametrize("func", [None, "tangence"])
+def test_past_the_caches(mt, rows, n, func):
+    """What tensors of 128 MiB and more get, on small ones: the same bits, in place too where there are many rows."""
+    x, gamma, beta, delta = inputs(rows + n, (rows, 1, n, 1), (1, 1, n, 1))
+    results = []
+    for option in (0, 1):
+        mt.set_option("nontemporal", option)
+        try:
+            out, mean, ivar, pk = run_forward(mt, x, gamma, beta, func, packed=True)
+            values = mt.CTensor(*x.shape)
+            mt.CTensorMath.Unpack(values, pk)
+            results.append([out, mean, ivar, values.numpy()])
+            for source in (x, pk):
+                for inplace in (False, True):
+                    results[-1] += run_backward(mt, delta, source, gamma, beta, mean, ivar, func, inplace=inplace).values()
+        finally:
+            mt.set_option("nontemporal", 2)
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
+    assert all(np.array_equal(results[0][k], results[0][k + 3]) for k in (4, 5, 6, 10, 11, 12))
+
+
+def test_squares_that_overflow(mt):
+    """Deviations above 1.8e19: no variance that fp32 holds, the row counts as having none of its values apart."""
+    for n in (100, 1024, 4096, 40000):
+        x = np.tile(np.float32([3e19, -3e19]), n // 2).reshape(1, 1, n, 1)
+        gamma, beta = np.full((1, 1, n, 1), 2, np.float32), np.full((1, 1, n, 1), 0.25, np.float32)
+        out, mean, ivar, _ = run_forward(mt, x, gamma, beta)
+        assert (out == 0.25).all() and mean.item() == 0 and ivar.item() == 0
+
+
 @pytest.mark.parametrize("func", ["sigmoid", "relu", "gelu", "leaky_relu", "linear", "tangence"])
 @pytest.mark.parametrize("n", [60, 1001, 2048, 20000, 40000])
 def test_functions(mt, func, n):

@@ -53,6 +53,23 @@ def test_pack_and_unpack(mt, shape):
     assert (np.abs(values.astype(np.float64) - x).reshape(shape[0], n) <= bound).all()
 
 
+@pytest.mark.parametrize("shape", [(3, 1, 128, 1), (5, 1, 1000, 1), (7, 3, 32, 32), (3, 1, 132, 1)])
+def test_past_the_caches(mt, shape):
+    """What tensors of 128 MiB and more get, on small ones: the same bits."""
+    x = Nrm(11, *shape)
+    got = []
+    for option in (0, 1):
+        mt.set_option("nontemporal", option)
+        try:
+            pk, back = mt.CPackedTensor(*shape), mt.CTensor(*shape)
+            mt.CTensorMath.Pack(pk, up(mt, x))
+            mt.CTensorMath.Unpack(back, pk)
+            got.append([*raw(mt, pk), back.numpy()])
+        finally:
+            mt.set_option("nontemporal", 2)
+    assert all(np.array_equal(a, b) for a, b in zip(*got)) and np.array_equal(got[0][3], po.through_8_bits(x))
+
+
 @pytest.mark.parametrize("shift", [1, 2, 3])
 @pytest.mark.parametrize("n", [4, 128, 1000, 1001, 4096])
 def test_tensors_off_a_16_byte_boundary(mt, n, shift):

@@ -1,19 +1,28 @@
-// The linear layer's weight gradient from an input kept in 8 bits, on the bf16 matrix cores with fp32 results.
+// The linear layer's weight gradient from an input kept in 8 bits, on the 16-bit matrix cores with fp32 results.
 //
 //   dweight[o][i] = sum_b delta[b][o] * (low[b][g] + step[b][g] * q[b][i]),  g = the group of 128 columns that i is in
 //                 = sum_b (delta * step)[b][o] * (q[b][i] - 128)  +  sum_b delta[b][o] * (low + 128 * step)[b][g]
 //
-// q - 128 is a whole number of 8 bits: exact in bf16.  delta * step, one fp32 product, is the exact sum of three bf16 numbers:
-// its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder exact; products below
-// 2^-110 lose the bits that no normal bf16 number holds).  Three bf16
-// matrix instructions therefore multiply what one fp32 product would, into fp32 accumulators, at a third of the bf16
-// rate (some 800 TFLOP/s) where the fp32 matrix instructions reach 157.  The second sum is one fp32 multiply-add per element of
+// q - 128 is a whole number of 8 bits: exact in 16 bits.  delta * step, one fp32 product, is written as a sum of 16-bit numbers, whose
+// products with q - 128 the matrix cores add up in fp32, in one of two ways.
+//   Three bf16 numbers: its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder
+//   exact; products below 2^-110 lose the bits that no normal bf16 number holds).
+//   Two fp16 numbers, rounded: the first off by at most 2^-12 of the product, the second by 2^-12 of that: 2^-24, the rounding of an
+//   fp32 product.  fp16 has little range: powers of two per row of dweight (of the largest delta) and per group (of the largest step)
+//   bring all products below 2^15, and small ones are off by 2^-25, nothing beside the rounding of the row's largest as long as
+//   that is not small itself.  The block checks that, and starts again with three numbers where it is not so.  The powers need a
+//   look at all of delta before (a launch that reads it once and sums the columns for dbias on the way), so this is for products that
+//   are worth it.
+// Three (two) 16-bit matrix instructions multiply what one fp32 product would, at a third (half) of a rate where the library's bf16
+// product reaches 1295 TFLOP/s; the fp32 matrix instructions reach 157 at most.  4096^3: 315 to 337 us in two numbers, 366 to 398 in
+// three (a chip that draws less power is faster: the clock falls to 1.9 GHz in these loops, and the matrix instructions of one wavefront
+// and the vector instructions of the other add up to 94 % of the cycles).  The second sum is one fp32 multiply-add per element of
 // delta on the way.
 //
 // A column tile is one group, so that a sample has one (low, step) in it.  A block is four wavefronts, each with its own 32 or
 // 64 rows (output features) and all 128 columns: no other wavefront needs its rows, so delta goes from memory to registers in
 // the lane layout of the matrix instruction and is scaled and cut there, never through LDS.  The columns, which all four
-// need, are turned into bf16 once and shared through LDS, eight samples of one column per 16 bytes: that is what a lane
+// need, are turned into 16-bit numbers once and shared through LDS, eight samples of one column per 16 bytes: that is what a lane
 // reads.  The block takes 64 samples per step; the next step's columns are loaded before and written after the step's
 // products, the next 16 samples of delta are loaded before the products of the 16 in hand.
 #include "mt_packed.h"
@@ -28,6 +37,9 @@ constexpr int THREADS = 256;    // of one group of four wavefronts
 constexpr uint32_t KSTEP = 64;  // samples per step
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
@@ -42,6 +54,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void *p, int l
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) {  // the bf16 numbers of a (low half) and b, cut off
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
+__device__ __forceinline__ uint32_t halves_of(float a, float b) {  // a (low half) and b rounded to fp16
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{a, b}), halfx2));
+}
+// The power of two of a largest magnitude, between 2^-126 and 2^126; 0 for an infinity, whose row is lost anyway
+__device__ __forceinline__ int exponent_of(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23) - 127;
+  return e == 128 ? 0 : max(-126, min(e, 126));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // e from -126 to 127
 __device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 
 struct WgradArgs {
@@ -50,19 +71,26 @@ struct WgradArgs {
   float *dweight, *dbias;    // split == 1: the gradients; else [split][Out*In] and [split][Out] partial sums
   uint32_t Out, tiles_m, split, per_split;  // per_split: samples of one part, a multiple of KSTEP
   bool accumulate;
+  // of a look at delta before (HALVES), over each part of the samples: [parts][Out + groups] largest magnitudes of delta and of the steps,
+  // [parts][Out] sums of delta
+  const float *ranges, *column_sums;
+  uint32_t parts;
+  bool accumulate_bias;
 };
 
 template <int TM>
 struct WgradSums {
   floatx16 acc[TM][4];           // matrix-core sums: 32 rows x 32 columns each
   float offset[TM], bias[TM];    // the second sum and the sum of delta: row lane % 32, half of the samples each
+  uint32_t seen[TM];             // the bits of all first fp16 numbers of a row
 };
 
 // the product over the samples k0 ... k1 (`steps` steps; those behind k1 add nothing).  The sum of delta is taken by all blocks though only those of the first group need it:
 // one addition in ten, where a second copy of the loop made those blocks the last ones (and the kernel's code twice as long).
-template <int TM>
+// HALVES: in two fp16 numbers; `row` and `step_scale` are the powers of two that bring delta * step below 2^15
+template <int TM, bool HALVES, bool BIAS>
 __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g, uint32_t m0, uint32_t k0, uint32_t k1, uint32_t steps, uintx4 (*cols)[KSTEP / 8][128],
-                                                  float2 (*scale)[KSTEP], WgradSums<TM> &sums) {
+                                                  float2 (*scale)[KSTEP], const float (&row)[TM], float step_scale, WgradSums<TM> &sums) {
   const uint32_t tid = threadIdx.x % THREADS, lane = tid & 63u, r = lane & 31u, half = lane >> 5;
   // this lane's rows r * TM ... of eight samples, AHEAD times 16 samples ahead of the products: 16 where two row tiles fill the
   // registers (two wavefronts per SIMD hide the rest), a whole step where there is room and often one wavefront
@@ -99,15 +127,24 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
   auto store_cols = [&](uint32_t buf) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = (float)((q[j] >> (8 * c)) & 255u) - 128.f;
       uintx4 w;
+      if constexpr (HALVES) {
+        // bytes under the exponent of 1024 are 1024 + q: less 1152, exact
 #pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = upper_halves(v[2 * j], v[2 * j + 1]);
+        for (int j = 0; j < 4; j++) {
+          const uint32_t t = __builtin_amdgcn_perm(q[2 * j + 1], q[2 * j], 0x0c040c00u + 0x00010001u * c) | 0x64006400u;
+          w[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, t) - (halfx2)(_Float16)1152.f);
+        }
+      } else {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = (float)((q[j] >> (8 * c)) & 255u) - 128.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = upper_halves(v[2 * j], v[2 * j + 1]);
+      }
       cols[buf][kg][c4 + c] = w;
     }
-    if (tid < KSTEP) scale[buf][tid] = make_float2(__uint_as_float(pair.y), __builtin_fmaf(128.f, __uint_as_float(pair.y), __uint_as_float(pair.x)));
+    if (tid < KSTEP) scale[buf][tid] = make_float2(__uint_as_float(pair.y) * step_scale, __builtin_fmaf(128.f, __uint_as_float(pair.y), __uint_as_float(pair.x)));
   };
 
   load_cols(k0);
@@ -121,38 +158,63 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
     float offset[TM] = {}, bias[TM] = {};  // of this step: sums of sums keep their error at the root of 32 and of the steps
 #pragma unroll
     for (int kk = 0; kk < 4; kk++) {
-      bf16x8 col[4];
+      uintx4 col[4];
 #pragma unroll
-      for (int n = 0; n < 4; n++) col[n] = __builtin_bit_cast(bf16x8, cols[buf][kk * 2 + half][n * 32 + r]);
+      for (int n = 0; n < 4; n++) col[n] = cols[buf][kk * 2 + half][n * 32 + r];
 #pragma unroll
       for (int m = 0; m < TM; m++) {
-        uintx4 cuts[3];
+        constexpr int CUTS = HALVES ? 2 : 3;
+        uintx4 cuts[CUTS];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           float x[2], y[2], z[2];
+          halfx2 h, l;
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const float v = d[kk % AHEAD][2 * j + e][m];
             const float2 sc = scale[buf][kk * 16 + half * 8u + 2 * j + e];
-            bias[m] += v;
+            if constexpr (BIAS) bias[m] += v;
             offset[m] = __builtin_fmaf(v, sc.y, offset[m]);
-            x[e] = v * sc.x;
-            y[e] = x[e] - cut(x[e]);
-            z[e] = y[e] - cut(y[e]);
+            if constexpr (HALVES) {
+              // (a fused product and sum of fp32 and fp16 numbers, rounded to fp16, is one instruction)
+              x[e] = v * row[m];
+              y[e] = sc.x;
+            } else {
+              x[e] = v * sc.x;
+              y[e] = x[e] - cut(x[e]);
+              z[e] = y[e] - cut(y[e]);
+            }
           }
-          cuts[0][j] = upper_halves(x[0], x[1]);
-          cuts[1][j] = upper_halves(y[0], y[1]);
-          cuts[2][j] = upper_halves(z[0], z[1]);
+          if constexpr (HALVES) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) h[e] = (_Float16)__builtin_fmaf(x[e], y[e], 0.f);
+            uint32_t first = __builtin_bit_cast(uint32_t, h);
+            asm volatile("" : "+v"(first));  // (the compiler would compute the second number again, into a low half)
+            h = __builtin_bit_cast(halfx2, first);
+            cuts[0][j] = first;
+            sums.seen[m] |= first;
+#pragma unroll
+            for (int e = 0; e < 2; e++) l[e] = (_Float16)__builtin_fmaf(x[e], y[e], -(float)h[e]);
+            cuts[1][j] = __builtin_bit_cast(uint32_t, l);
+          } else {
+            cuts[0][j] = upper_halves(x[0], x[1]);
+            cuts[1][j] = upper_halves(y[0], y[1]);
+            cuts[CUTS - 1][j] = upper_halves(z[0], z[1]);
+          }
         }
         // (the compiler would leave these sums for the end of the step and keep four times the registers of delta for them)
         asm volatile("" : "+v"(offset[m]));
-        asm volatile("" : "+v"(bias[m]));
+        if constexpr (BIAS) asm volatile("" : "+v"(bias[m]));
         if (m == TM - 1) load_delta(k + 16u * (kk + AHEAD), d[kk % AHEAD]);
 #pragma unroll
-        for (int p = 0; p < 3; p++)
+        for (int p = 0; p < CUTS; p++)
 #pragma unroll
-          for (int n = 0; n < 4; n++)
-            sums.acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, cuts[p]), col[n], sums.acc[m][n], 0, 0, 0);
+          for (int n = 0; n < 4; n++) {
+            if constexpr (HALVES)
+              sums.acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, cuts[p]), __builtin_bit_cast(halfx8, col[n]), sums.acc[m][n], 0, 0, 0);
+            else
+              sums.acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, cuts[p]), __builtin_bit_cast(bf16x8, col[n]), sums.acc[m][n], 0, 0, 0);
+          }
       }
       __builtin_amdgcn_sched_barrier(0);  // nothing of the next 16 samples moves up: the registers are full
     }
@@ -167,8 +229,9 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
 }
 
 // Stores column tiles N0 ... N1 of a wavefront's sums
-template <int TM, int N0, int N1>
-__device__ __forceinline__ void packed_wgrad_store(const WgradArgs &a, float *dw, uint32_t g, uint32_t m0, const float4 (*offsets)[8], const WgradSums<TM> &sums) {
+template <int TM, int N0, int N1, bool HALVES>
+__device__ __forceinline__ void packed_wgrad_store(const WgradArgs &a, float *dw, uint32_t g, uint32_t m0, const float4 (*offsets)[8], const int4 (*powers)[8],
+                                                   const WgradSums<TM> &sums) {
   const uint32_t lane = threadIdx.x & 63u, r = lane & 31u, half = lane >> 5;
   // accumulator i of tile (m, n): row 8 * (i / 4) + 4 * half + i % 4, column 32 * n + r.  Rows and columns that do not exist have
   // offsets behind the end of the buffer: their stores are dropped
@@ -187,12 +250,14 @@ __device__ __forceinline__ void packed_wgrad_store(const WgradArgs &a, float *dw
     for (int m = 0; m < TM; m++) {
       const float4 c4 = offsets[m][i4 * 2 + half];
       const float c[4] = {c4.x, c4.y, c4.z, c4.w};
+      const int4 p4 = HALVES ? powers[m][i4 * 2 + half] : int4{};
+      const int power[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const uint32_t row = (i * TM + m) * row_bytes;
         float v[4];
 #pragma unroll
-        for (int n = N0; n < N1; n++) v[n] = sums.acc[m][n][i4 * 4 + i] + c[i];
+        for (int n = N0; n < N1; n++) v[n] = (HALVES ? __builtin_amdgcn_ldexpf(sums.acc[m][n][i4 * 4 + i], power[i]) : sums.acc[m][n][i4 * 4 + i]) + c[i];
         if (a.accumulate) {
 #pragma unroll
           for (int n = N0; n < N1; n++) v[n] += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(voff[n] + row), 0, 0));
@@ -207,11 +272,12 @@ __device__ __forceinline__ void packed_wgrad_store(const WgradArgs &a, float *dw
 // KW groups of four wavefronts per block.  Two groups take half of the block's samples each, with their own columns in LDS, and add
 // their sums at the end: where the tiles are few, the second wavefront per SIMD that fills the first one's waits comes from the
 // same tile instead of from another part of the batch, whose sums would go through memory.
-template <int TM, int KW>
+template <int TM, int KW, bool HALVES>
 __global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(WgradArgs a) {
   __shared__ uintx4 cols[KW][2][KSTEP / 8][128];  // [eight samples][column]
   __shared__ float2 scale[KW][2][KSTEP];          // (step, low + 128 * step)
   __shared__ float4 offsets[4][TM][8];            // the second sum of every row of a wavefront
+  __shared__ int4 powers[HALVES ? 4 : 1][TM][8];    // the power of two that its products lack
   __shared__ float halves[KW > 1 ? 2 : 1][4][TM][32];
   const uint32_t lane = threadIdx.x & 63u, r = lane & 31u, half = lane >> 5;
   const uint32_t kw = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u % 4u);
@@ -222,21 +288,91 @@ __global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(Wgra
   const uint32_t m0 = (t % a.tiles_m) * (128u * TM) + wave * (32u * TM), part = t / a.tiles_m;
   const uint32_t k0 = part * a.per_split, k1 = min(a.in.w, k0 + a.per_split);
   const uint32_t steps = ((k1 - k0 + KSTEP - 1) / KSTEP + KW - 1) / KW;  // of each group
-  const bool bias = a.dbias != nullptr && g == 0;
+  const bool bias = a.dbias != nullptr && g == 0 && (!HALVES || part == 0);
   WgradSums<TM> sums;
+  const auto clear = [&] {
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      sums.offset[m] = 0.f;
+#pragma unroll
+      for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
+    }
+  };
+  clear();
 #pragma unroll
   for (int m = 0; m < TM; m++) {
-    sums.offset[m] = sums.bias[m] = 0.f;
-#pragma unroll
-    for (int n = 0; n < 4; n++) sums.acc[m][n] = 0.f;
+    sums.bias[m] = 0.f;
+    sums.seen[m] = 0u;
   }
   const uint32_t first = min(k1, k0 + kw * steps * KSTEP), last = min(k1, first + steps * KSTEP);
-  packed_wgrad_loop<TM>(a, g, m0, first, last, steps, cols[kw], scale[kw], sums);
+  if constexpr (HALVES) {
+    __shared__ uint32_t seen[KW][4][TM][32];
+    float most[TM] = {}, most_step = 0.f;
+    const uint32_t stride = a.Out + a.in.groups;
+    uint32_t o[TM];
+#pragma unroll
+    for (int m = 0; m < TM; m++) o[m] = min(m0 + r * TM + m, a.Out - 1);
+    for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) {
+        const float *ranges = a.ranges + (size_t)min(p0 + u, a.parts - 1) * stride;
+#pragma unroll
+        for (int m = 0; m < TM; m++) most[m] = fmaxf(most[m], ranges[o[m]]);
+        most_step = fmaxf(most_step, ranges[a.Out + g]);
+      }
+    }
+    if (bias && kw == 0 && half == 0) {
+      for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
+        float t[8][TM];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++)
+#pragma unroll
+          for (int m = 0; m < TM; m++) t[u][m] = p0 + u < a.parts ? a.column_sums[(size_t)(p0 + u) * a.Out + o[m]] : 0.f;
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++)
+#pragma unroll
+          for (int m = 0; m < TM; m++) sums.bias[m] += t[u][m];
+      }
+    }
+    const int step_power = min(127, 12 - exponent_of(most_step));
+    float row[TM];
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      const int e = exponent_of(most[m]);
+      row[m] = power_of_two(-e);
+      if (kw == 0 && half == 0) reinterpret_cast<int *>(powers[wave][m])[r] = e - step_power;
+    }
+    packed_wgrad_loop<TM, true, false>(a, g, m0, first, last, steps, cols[kw], scale[kw], row, power_of_two(step_power), sums);
+    // Was every row's largest product near the product of the largest delta and the largest step?  A first number of 2 or more (the upper
+    // exponent bit) says so: what a smaller one of its row lacks is at most 2^-26 of it.  If not (a sample of huge values that has no
+    // delta, say), the block starts again with the three numbers that have fp32's range
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+      sums.seen[m] |= __shfl_xor(sums.seen[m], 32, 64);
+      seen[kw][wave][m][r] = sums.seen[m];
+    }
+    __syncthreads();
+    bool good = true;
+#pragma unroll
+    for (int m = 0; m < TM; m++) good = good && (most[m] == 0.f || most_step == 0.f || ((seen[0][wave][m][r] | seen[KW - 1][wave][m][r]) & 0x40004000u) != 0u);
+    if (!__syncthreads_and(good)) {
+      clear();
+#pragma unroll
+      for (int m = 0; m < TM; m++) {
+        row[m] = 1.f;
+        if (kw == 0 && half == 0) reinterpret_cast<int *>(powers[wave][m])[r] = 0;
+      }
+      packed_wgrad_loop<TM, false, false>(a, g, m0, first, last, steps, cols[kw], scale[kw], row, 1.f, sums);
+    }
+  } else {
+    const float row[TM] = {};
+    packed_wgrad_loop<TM, false, true>(a, g, m0, first, last, steps, cols[kw], scale[kw], row, 1.f, sums);
+  }
 
   float *dw = a.dweight, *db = a.dbias;
   if (a.split > 1) {
     dw += (size_t)part * a.Out * a.in.n;
-    if (bias) db += (size_t)part * a.Out;
+    if (bias && !HALVES) db += (size_t)part * a.Out;
   }
   float c[TM], sum[TM];
 #pragma unroll
@@ -282,18 +418,42 @@ __global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(Wgra
       reinterpret_cast<float *>(offsets[wave][m])[r] = c[m];
       if (bias && m0 + r * TM + m < a.Out) {
         float *p = db + m0 + r * TM + m;
-        *p = a.accumulate ? *p + sum[m] : sum[m];
+        *p = (HALVES ? a.accumulate_bias : a.accumulate) ? *p + sum[m] : sum[m];
       }
     }
   }
   __syncthreads();
   if constexpr (KW == 1) {
-    packed_wgrad_store<TM, 0, 4>(a, dw, g, m0, offsets[wave], sums);
+    packed_wgrad_store<TM, 0, 4, HALVES>(a, dw, g, m0, offsets[wave], powers[HALVES ? wave : 0], sums);
   } else if (kw == 0) {
-    packed_wgrad_store<TM, 0, 2>(a, dw, g, m0, offsets[wave], sums);
+    packed_wgrad_store<TM, 0, 2, HALVES>(a, dw, g, m0, offsets[wave], powers[HALVES ? wave : 0], sums);
   } else {
-    packed_wgrad_store<TM, 2, 4>(a, dw, g, m0, offsets[wave], sums);
+    packed_wgrad_store<TM, 2, 4, HALVES>(a, dw, g, m0, offsets[wave], powers[HALVES ? wave : 0], sums);
   }
+}
+
+// the largest magnitude (a NaN counts as none) of every column of delta, then of the steps of every group, over `per_part` samples, and
+// the columns' sums
+__global__ __launch_bounds__(THREADS) void packed_wgrad_ranges_kernel(float *ranges, float *sums, const float *delta, PackedView in, uint32_t Out, uint32_t per_part) {
+  const uint32_t i = blockIdx.x * THREADS + threadIdx.x, k0 = blockIdx.y * per_part, count = min(per_part, in.w - k0);
+  if (i >= Out + in.groups) return;
+  const bool steps = i >= Out;
+  const size_t stride = steps ? (size_t)in.groups * 2 : Out;
+  const float *p = steps ? &in.pair[(size_t)k0 * in.groups + (i - Out)].y : delta + (size_t)k0 * Out + i;
+  float most = 0.f, sum = 0.f;
+  for (uint32_t k = 0; k < count; k += 16) {
+    float t[16], s = 0.f;
+#pragma unroll
+    for (uint32_t u = 0; u < 16; u++) t[u] = p[(size_t)min(k + u, count - 1) * stride];
+#pragma unroll
+    for (uint32_t u = 0; u < 16; u++) {
+      most = fmaxf(most, fabsf(t[u]));
+      s += k + u < count ? t[u] : 0.f;
+    }
+    sum += s;
+  }
+  ranges[(size_t)blockIdx.y * (Out + in.groups) + i] = most;
+  if (!steps) sums[(size_t)blockIdx.y * Out + i] = sum;
 }
 
 // the parts of a split sum, in a fixed order: first the weights' n values, then the bias's Out; SLICES threads per value, which take
@@ -339,18 +499,22 @@ __global__ __launch_bounds__(THREADS) void bias_only_kernel(float *dbias, const 
 
 mt::Workspace g_wgrad_ws;
 
-// The variant: rows per block (256: each sample's columns are turned into bf16 for twice the products; 128: twice the blocks), one or
+// The variant: rows per block (256: each sample's columns are turned into 16-bit numbers for twice the products; 128: twice the blocks), one or
 // two groups of wavefronts per block, parts of the batch.  The estimate of each variant's time in microseconds is its fixed part plus
 // the steps that the busiest compute unit takes, at the measured time of a step with one or two blocks on it, plus writing and
-// joining the parts' sums.  Measured against one another: 4096^3 366 us with 256 rows, 412 with 128; 2048^3 58 with 128 rows and
-// two groups, 66 with one, 72 with 256 rows and four parts; 1000 x 1000 x 1777 27.5 with two groups, 31.9 with two parts; 512^3 11.2 in
-// four parts, 19 in one.
+// joining the parts' sums; two fp16 numbers instead of three bf16 ones take 0.82 of the steps' time and a look at delta before.  Measured
+// against one another, in three numbers: 4096^3 366 us with 256 rows, 412 with 128; 2048^3 58 with 128 rows and two groups, 66 with one,
+// 72 with 256 rows and four parts; 1000 x 1000 x 1777 27.5 with two groups, 31.9 with two parts; 512^3 11.2 in four parts, 19 in
+// one.  In two numbers against three (on a slower chip): 4096^3 337 and 383, 8192 x 4096 x 1024 186 and 214, 2048^3 54.8 and 58.6,
+// 256 x 4096 x 4096 33.6 and 33.4, 512^3 15.3 and 11.2.
 struct Plan {
   uint32_t rows, split;
-  bool pair;
+  bool pair, half;
 };
-Plan choose(uint32_t Out, uint32_t groups, uint32_t steps, size_t n) {
-  Plan best{128, 1, false};
+Plan choose(uint32_t Out, uint32_t groups, uint32_t samples, size_t n) {
+  const uint32_t steps = cdiv(samples, KSTEP);
+  const double look = 4.0 + (double)samples * Out * 4 / 5.6e6;  // what the launch before and its results cost
+  Plan best{128, 1, false, false};
   double least = 1e30;
   for (int kind = 0; kind < 3; kind++) {
     const uint32_t rows = kind == 2 ? 256 : 128;
@@ -364,10 +528,12 @@ Plan choose(uint32_t Out, uint32_t groups, uint32_t steps, size_t n) {
       const size_t rest = blocks % 512;
       const double turn = blocks / 512 * two + (rest > 256 ? two : rest > 0 ? one : 0.0);
       const uint32_t each = cdiv(cdiv(steps, split), pair ? 2 : 1);
-      const double us = fixed + each * turn + (split > 1 ? 4.0 + split * (double)n * 2e-6 : 0.0);
+      const double rest_us = fixed + (split > 1 ? 4.0 + split * (double)n * 2e-6 : 0.0), loop_us = each * turn;
+      const bool half = kind != 0 && 0.82 * loop_us + look < loop_us;  // (kind 0 is for few steps)
+      const double us = rest_us + (half ? 0.82 * loop_us + look : loop_us);
       if (us < least) {
         least = us;
-        best = Plan{rows, split, pair};
+        best = Plan{rows, split, pair, half};
       }
     }
   }
@@ -412,20 +578,37 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   WgradArgs a{};
   a.delta = delta->p; a.in = v; a.Out = Out; a.accumulate = accumulate != 0;
   const size_t n = (size_t)Out * v.n;
-  const uint32_t steps = cdiv(v.w, KSTEP);
-  const Plan plan = choose(Out, v.groups, steps, n);
+  const Plan plan = choose(Out, v.groups, v.w, n);
   const bool wide = plan.rows == 256, pair = plan.pair;
   const uint32_t split = plan.split;
   a.tiles_m = cdiv(Out, plan.rows);
   const size_t tiles = (size_t)a.tiles_m * v.groups;
   a.per_split = cdiv(cdiv(v.w, split), KSTEP) * KSTEP;
   a.split = cdiv(v.w, a.per_split);
+  const uint32_t columns = Out + v.groups, column_blocks = cdiv(columns, THREADS);
+  uint32_t parts = 0, per_part = 0;
+  if (plan.half) {
+    // enough blocks for the whole chip, parts of at least 32 samples, few enough for every thread to read them all
+    parts = cdiv(512, column_blocks);
+    parts = parts > 32 ? 32 : parts;
+    per_part = cdiv(v.w, parts) < 32 ? 32 : cdiv(v.w, parts);
+    parts = cdiv(v.w, per_part);
+  }
+  const size_t sums = a.split > 1 ? a.split * (n + Out) : 0, ranges = (size_t)parts * columns, column_sums = (size_t)parts * Out;
   float *ws = nullptr;
-  if (a.split > 1) {
-    int rc = mt::workspace_get(g_wgrad_ws, "packed weight gradient", a.split * (n + Out), &ws);
+  if (sums + ranges) {
+    int rc = mt::workspace_get(g_wgrad_ws, "packed weight gradient", sums + ranges + column_sums, &ws);
     if (rc) return rc;
+  }
+  if (plan.half) {
+    a.ranges = ws + sums;
+    a.column_sums = a.ranges + ranges;
+    a.parts = parts;
+    a.accumulate_bias = a.accumulate;
+  }
+  if (a.split > 1) {
     a.dweight = ws;
-    a.dbias = dbias ? ws + a.split * n : nullptr;
+    a.dbias = !dbias ? nullptr : plan.half ? dbias->p : ws + a.split * n;
     a.accumulate = false;
   } else {
     a.dweight = dweight->p;
@@ -433,15 +616,20 @@ int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_ten
   }
   const size_t grid = tiles * a.split;
   if (grid >= (1u << 23)) return mt::fail(MT_E_UNAVAILABLE, "%s: too many weights for one launch", name);  // a grid has fewer than 2^32 threads
-  if (wide)
-    packed_wgrad_kernel<2, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  if (plan.half) packed_wgrad_ranges_kernel<<<dim3(column_blocks, parts), THREADS, 0, mt::stream()>>>(ws + sums, ws + sums + ranges, delta->p, v, Out, per_part);
+  if (wide && plan.half)
+    packed_wgrad_kernel<2, 1, true><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  else if (wide)
+    packed_wgrad_kernel<2, 1, false><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+  else if (pair && plan.half)
+    packed_wgrad_kernel<1, 2, true><<<(unsigned)grid, 2 * THREADS, 0, mt::stream()>>>(a);
   else if (pair)
-    packed_wgrad_kernel<1, 2><<<(unsigned)grid, 2 * THREADS, 0, mt::stream()>>>(a);
+    packed_wgrad_kernel<1, 2, false><<<(unsigned)grid, 2 * THREADS, 0, mt::stream()>>>(a);
   else
-    packed_wgrad_kernel<1, 1><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
+    packed_wgrad_kernel<1, 1, false><<<(unsigned)grid, THREADS, 0, mt::stream()>>>(a);
   MT_LAUNCH_CHECK(name);
   if (a.split > 1) {
-    float *db = dbias ? dbias->p : nullptr;
+    float *db = dbias && !plan.half ? dbias->p : nullptr;
     if (a.split > 8)
       packed_wgrad_join_kernel<4><<<cdiv(n + Out, THREADS / 4), THREADS, 0, mt::stream()>>>(dweight->p, db, ws, ws + a.split * n, a.split, n, Out, accumulate != 0);
     else

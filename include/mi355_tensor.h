@@ -440,9 +440,10 @@ int mt_unpack(const mt_tensor *output, const mt_packed_tensor *input);          
 /* CNetLayerLinear::TrainingBackward, weight and bias part (netlayer/cnetlayerlinear.cu.h:415-447), from an input kept in 8 bits:
  * dweight [1,1,Out,In] (+)= sum over the batch of delta (x) value(input), dbias [1,1,Out,1] (NULL to skip) (+)= sum of delta;
  * input [B,...] of In values per sample, delta [B,...] of Out values.  accumulate: 1 adds to what the gradients hold, 0 overwrites.
- * The products are those of the fp32 numbers delta and step with the whole numbers q, summed in fp32; a gradient's bits depend
- * on the sizes only.  A delta that is not a finite number, or whose product with a step is none, makes its row of dweight NaN in
- * the columns of that group.  Fewer than 2^24 features on either side. */
+ * delta*step is an fp32 number, or (large layers) one whose error is at most 2^-24 of itself or 2^-26 of the largest in its row of dweight;
+ * its products with the whole numbers q are exact and summed in fp32.  The same call gives the same bits.  A delta that is not a
+ * finite number, or whose product with a step is none, makes its row of dweight NaN in the columns that it meets.  Fewer than 2^24
+ * features on either side. */
 int mt_linear_backward_weights_sum_packed(const mt_tensor *dweight, const mt_tensor *dbias, const mt_packed_tensor *input, const mt_tensor *delta, int accumulate);
 
 /* TrainingResetDeltaWeight of every layer of a network (netlayer/cnetlayerconvolution.cu.h:522-526 and the same

@@ -140,6 +140,49 @@ def test_linear_large(mt, b, n_in, n_out):
     check_linear(mt, b, n_in, n_out, b)
 
 
+def unequal(x, delta, what):
+    """Magnitudes that 16 bits cannot hold beside one another."""
+    rng = np.random.default_rng(5)
+    if what == "samples without delta":        # as padding may leave them: huge activations, no gradient
+        x[3], delta[3] = x[3] * 1e30, 0
+        x[-1], delta[-1] = x[-1] * 1e12, 0
+    elif what == "samples with little delta":
+        x[3], delta[3] = x[3] * 1e10, delta[3] * 1e-10
+    elif what == "one feature's activations":
+        x[:, :, 5] *= 1e8
+    elif what == "every row":
+        delta *= np.exp(rng.uniform(-60, 60, (1, delta.shape[1], delta.shape[2], 1))).astype(np.float32)
+    elif what == "every sample":
+        x *= np.exp(rng.uniform(-25, 25, (x.shape[0], 1, 1, 1))).astype(np.float32)
+    elif what == "rows of zeros":
+        delta[:, :, ::3] = 0
+    elif what == "one sample of a row":
+        delta[:, :, 7] = 0
+        delta[11, :, 7] = 1e-20
+    elif what == "constant activations":
+        x[:, :, :128] = x[:, :, :1]
+
+
+# the first three are large enough for two fp16 numbers per product (256 rows per block, 128, an odd number of them in parts of the batch)
+@pytest.mark.parametrize("b,n_in,n_out", [(1100, 4000, 4000), (1500, 2000, 1500), (5000, 1000, 1501), (300, 257, 130)])
+@pytest.mark.parametrize("what", ["nothing", "samples without delta", "samples with little delta", "one feature's activations", "every row", "every sample",
+                                  "rows of zeros", "one sample of a row", "constant activations"])
+def test_linear_unequal_magnitudes(mt, b, n_in, n_out, what):
+    x, delta = Nrm(1, b, 1, n_in, 1), Nrm(2, b, 1, n_out, 1, std=0.02)
+    unequal(x, delta, what)
+    dw, db = run_linear(mt, x, delta)
+    want = po.linear_weights(delta.reshape(b, n_out), x)
+    for key, got in (("dweight", dw), ("dbias", db)):
+        assert (np.abs(got - want[key]) <= want[key + "_tol"] + 1e-44).all(), (key, float(np.max(np.abs(got - want[key]) / (want[key + "_tol"] + 1e-44))))
+    # and every row as a whole, as in check_linear
+    size = want["dweight_tol"] / (b + 18)
+    assert (np.linalg.norm(dw - want["dweight"], axis=1) <= 8 * np.linalg.norm(size, axis=1) + 1e-44).all()
+    again = run_linear(mt, x, delta)
+    assert np.array_equal(dw, again[0]) and np.array_equal(db, again[1])
+    added = run_linear(mt, x, delta, accumulate=True, start=(np.ones((1, 1, n_out, n_in), np.float32), np.ones((1, 1, n_out, 1), np.float32)))
+    assert np.array_equal(added[0], dw + np.float32(1)) and np.array_equal(added[1], db + np.float32(1))
+
+
 @pytest.mark.parametrize("b,n_in,n_out", [(5, 100, 30), (300, 257, 129), (4096, 128, 64), (64, 1024, 1024)])
 def test_linear_adds_and_repeats(mt, b, n_in, n_out):
     x, delta = Nrm(1, b, 1, n_in, 1), Nrm(2, b, n_out, 1, 1)      # delta seen as [B,Out,1,1]
@@ -152,7 +195,7 @@ def test_linear_adds_and_repeats(mt, b, n_in, n_out):
     assert np.array_equal(alone[0], fresh[0]) and (alone[1] == 7).all()
 
 
-@pytest.mark.parametrize("b,n_in,n_out", [(40, 300, 140), (3000, 130, 60)])
+@pytest.mark.parametrize("b,n_in,n_out", [(40, 300, 140), (3000, 130, 60), (1500, 2000, 1500), (1100, 4000, 4000)])
 def test_linear_values_that_are_not_finite(mt, b, n_in, n_out):
     x, delta = Nrm(1, b, 1, n_in, 1), Nrm(2, b, 1, n_out, 1)
     fine = run_linear(mt, x, delta)

@@ -69,48 +69,81 @@ __device__ __forceinline__ void apply(int func, float *v) {
   }
 }
 
-// ---- one step of a thread: one value, four neighbouring ones, or four past the caches, for tensors that are too large for them and
-// touched once (option "nontemporal": 128 MiB and more; 16384 x 4096 forward 102 -> 98 us, backward 148 -> 139).  A flag at run time does
-// not do: the compiler merges the two accesses into the ordinary one. -----------------------------------------------------------
-enum Access { ONE, FOUR, FOUR_PAST };
+// ---- one step of a thread: one value, or four neighbouring ones: from a 16-byte boundary, the same past the caches, for tensors that are
+// too large for them and touched once (option "nontemporal": 128 MiB and more; 16384 x 4096 forward 102 -> 98 us, backward 148 -> 139; a
+// flag at run time does not do: the compiler merges the two accesses into the ordinary one), or from any address, for rows of any
+// length (1344 x 10319 backward 73 us with single values, 59 so) ---------------------------------------------------------------------
+enum Access { ONE, FOUR, FOUR_PAST, FOUR_ANY };
+constexpr int kept(int access) { return access == FOUR_PAST ? FOUR : access; }  // for what is read again
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <int ACCESS>
-__device__ __forceinline__ void load_step(float *t, const float *p, uint32_t at) {
+__device__ __forceinline__ void load_step(float *t, const float *p, int at) {
   if (ACCESS == ONE) {
     t[0] = p[at];
   } else {
-    const floatx4 *q = reinterpret_cast<const floatx4 *>(p + at);
-    const floatx4 v = ACCESS == FOUR_PAST ? __builtin_nontemporal_load(q) : *q;
+    floatx4 v;
+    if (ACCESS == FOUR_ANY)
+      v = *reinterpret_cast<const floatx4_any *>(p + at);
+    else if (ACCESS == FOUR_PAST)
+      v = __builtin_nontemporal_load(reinterpret_cast<const floatx4 *>(p + at));
+    else
+      v = *reinterpret_cast<const floatx4 *>(p + at);
     t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
   }
 }
+// `left`: values from p to the end
 template <int ACCESS>
-__device__ __forceinline__ void store_step(float *p, const float *t) {
+__device__ __forceinline__ void store_step(float *p, const float *t, uint32_t left) {
   if (ACCESS == ONE) {
     *p = t[0];
   } else {
     const floatx4 v = {t[0], t[1], t[2], t[3]};
     if (ACCESS == FOUR_PAST)
       __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(p));
-    else
+    else if (ACCESS == FOUR)
       *reinterpret_cast<floatx4 *>(p) = v;
+    else if (left >= 4)
+      *reinterpret_cast<floatx4_any *>(p) = v;
+    else
+#pragma unroll
+      for (uint32_t e = 0; e < 3; e++)
+        if (e < left) p[e] = t[e];
+  }
+}
+// Where the step that starts at `first` of N values loads: steps that would pass the end load the last four (a piece of fewer than four
+// reaches into the piece before), and are then moved into place
+template <int ACCESS>
+__device__ __forceinline__ int load_at(uint32_t first, uint32_t N) { return min((int)first, (int)N - (ACCESS == ONE ? 1 : 4)); }
+template <int ACCESS>
+__device__ __forceinline__ void settle(float *t, uint32_t first, uint32_t N) {
+  if (ACCESS == FOUR_ANY) {
+    const uint32_t by = first < N && first + 4 > N ? first + 4 - N : 0u;  // 0 to 3
+    const float a = t[0], b = t[1], c = t[2], d = t[3];  // (selects between elements of an array would put it into memory)
+    t[0] = by == 0 ? a : by == 1 ? b : by == 2 ? c : d;
+    t[1] = by == 0 ? b : by == 1 ? c : by == 2 ? d : 0.f;
+    t[2] = by == 0 ? c : by == 1 ? d : 0.f;
+    t[3] = by == 0 ? d : 0.f;
   }
 }
 
 // ---- how the L threads of a row share its N values: E each, in vectors of four 4 * L apart, or singly L apart ----------------
-template <int L, int E, bool VEC>
+template <int L, int E, int ACCESS>
 struct Share {
-  static constexpr int STEPS = VEC ? E / 4 : E, WIDTH = VEC ? 4 : 1;
+  static constexpr int STEPS = ACCESS != ONE ? E / 4 : E, WIDTH = ACCESS != ONE ? 4 : 1;
   static __device__ __forceinline__ uint32_t first(int j) { return (j * L + threadIdx.x % L) * WIDTH; }
-  // values behind the end read the last ones again and count as 0
-  template <int ACCESS = VEC ? FOUR : ONE>
+  static __device__ __forceinline__ bool inside(int j, int e, uint32_t N) { return first(j) + (ACCESS == FOUR_ANY ? e : 0) < N; }
+  // values behind the end count as 0
+  template <int HOW = kept(ACCESS)>
   static __device__ __forceinline__ void load(float (&v)[E], const float *p, uint32_t N) {
 #pragma unroll
-    for (int j = 0; j < STEPS; j++) load_step<ACCESS>(v + j * WIDTH, p, min(first(j), N - WIDTH));
+    for (int j = 0; j < STEPS; j++) load_step<HOW>(v + j * WIDTH, p, load_at<HOW>(first(j), N));
 #pragma unroll
-    for (int j = 0; j < STEPS; j++)
+    for (int j = 0; j < STEPS; j++) {
+      settle<HOW>(v + j * WIDTH, first(j), N);
 #pragma unroll
       for (int e = 0; e < WIDTH; e++) v[j * WIDTH + e] = first(j) < N ? v[j * WIDTH + e] : 0.f;
+    }
   }
 };
 
@@ -118,6 +151,7 @@ struct Share {
 // decoding are two steps, so that all loads of a row are under way before the first is waited for ------------------------------
 struct RowsF32 {
   static constexpr int BYTES = 4;  // of a value, about
+  bool in_fours() const { return true; }
   const float *p;
   uint32_t N;
   template <bool VEC>
@@ -131,14 +165,19 @@ struct RowsF32 {
   struct Row {
     const float *p;
     template <int ACCESS>
-    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, uint32_t at) const { load_step<ACCESS>(raw.t, p, at); }
+    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, int at) const { load_step<ACCESS>(raw.t, p, at); }
   };
+  template <int ACCESS>
+  static __device__ __forceinline__ int at(uint32_t first, uint32_t N) { return load_at<ACCESS>(first, N); }
+  template <int ACCESS>
+  static __device__ __forceinline__ void settle_values(float *x, uint32_t first, uint32_t N) { settle<ACCESS>(x, first, N); }
   __device__ __forceinline__ Row row(uint32_t r) const { return Row{p + (size_t)r * N}; }
 };
 struct RowsPacked {
   static constexpr int BYTES = 1;
   PackedView v;
   uint32_t N, per_sample;  // rows of one sample
+  bool in_fours() const { return N % 4 == 0 || per_sample == 1; }  // do four neighbouring values lie in one group
   template <bool VEC>
   struct Raw {
     float2 pair;
@@ -153,29 +192,39 @@ struct RowsPacked {
     const float2 *pair;
     uint32_t first;  // the row's first value within its sample
     template <int ACCESS>
-    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, uint32_t at) const {
+    __device__ __forceinline__ void load(Raw<ACCESS != ONE> &raw, int at) const {
       const uint32_t e = first + at;
       raw.pair = pair[e / mt::PACK_GROUP];
       raw.q = ACCESS != ONE ? *reinterpret_cast<const uint32_t *>(q + e) : q[e];
     }
   };
+  // (four bytes of one group, from a multiple of four: those behind a sample's end are its padding)
+  template <int ACCESS>
+  static __device__ __forceinline__ int at(uint32_t first, uint32_t N) { return ACCESS == ONE ? min(first, N - 1) : min(first, (N - 1) & ~3u); }
+  template <int ACCESS>
+  static __device__ __forceinline__ void settle_values(float *, uint32_t, uint32_t) {}
   __device__ __forceinline__ Row row(uint32_t r) const {
     const uint32_t w = per_sample == 1 ? r : r / per_sample;
     return Row{v.q + (size_t)w * v.pitch, v.pair + (size_t)w * v.groups, (r - w * per_sample) * N};
   }
 };
 
-// the 8 bits of one vector per lane, 32 lanes a group: lanes behind the end of the row give
-// `valid` false; those behind the end of the sample write its padding
-__device__ __forceinline__ void pack_step(const PackedView &out, size_t sample, uint32_t e, bool valid, const float *t) {
-  float low = mt::min_nan(mt::min_nan(t[0], t[1]), mt::min_nan(t[2], t[3])), high = mt::max_nan(mt::max_nan(t[0], t[1]), mt::max_nan(t[2], t[3]));
+// the 8 bits of one vector per lane, 32 lanes a group: a lane's first `left` values are the row's; lanes behind the end of the sample
+// write its padding
+__device__ __forceinline__ void pack_step(const PackedView &out, size_t sample, uint32_t e, int left, const float *t) {
+  const bool valid = left > 0;
+  float u[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) u[k] = k < left ? t[k] : t[0];
+  float low = mt::min_nan(mt::min_nan(u[0], u[1]), mt::min_nan(u[2], u[3])), high = mt::max_nan(mt::max_nan(u[0], u[1]), mt::max_nan(u[2], u[3]));
   low = mt::over_lanes<mt::Lowest, 32>(valid ? low : __int_as_float(0x7f800000));
   high = mt::over_lanes<mt::Highest, 32>(valid ? high : __int_as_float(0xff800000));
   const mt::PackScale s = mt::pack_scale(low, high);
   uint32_t w = 0;
 #pragma unroll
-  for (int k = 0; k < 4; k++) w = mt::pack_into(s, t[k], k, w);
-  if (valid || (e >= out.n && e < out.pitch)) *reinterpret_cast<uint32_t *>(out.q + sample * out.pitch + e) = valid ? w : 0u;
+  for (int k = 0; k < 4; k++) w = mt::pack_into(s, u[k], k, w);
+  if (left < 4) w &= valid ? (1u << 8 * left) - 1u : 0u;
+  if (valid || (e >= out.n && e < out.pitch)) *reinterpret_cast<uint32_t *>(out.q + sample * out.pitch + e) = w;
   if (valid && e % mt::PACK_GROUP == 0) out.pair[sample * out.groups + e / mt::PACK_GROUP] = make_float2(s.low, s.step);
 }
 
@@ -192,9 +241,9 @@ struct Forward {
 
 // gamma and beta of a thread's share of a row: in registers, or loaded where they are used (1024 threads with 32 values of x each
 // have no registers for them: 1000 x 32768 61 us, 65 with them)
-template <int L, int E, bool VEC>
+template <int L, int E, int ACCESS>
 struct Parameters {
-  using S = Share<L, E, VEC>;
+  using S = Share<L, E, ACCESS>;
   static constexpr bool HELD = E <= 16;
   float gamma[HELD ? E : 1], beta[HELD ? E : 1];
   __device__ __forceinline__ void load(const float *g, const float *b, uint32_t N) {
@@ -203,7 +252,7 @@ struct Parameters {
       S::load(beta, b, N);
     }
   }
-  __device__ __forceinline__ void step(const float *g, const float *b, int j, float *tg, float *tb) const {
+  __device__ __forceinline__ void step(const float *g, const float *b, int j, uint32_t N, float *tg, float *tb) const {
     if constexpr (HELD) {
 #pragma unroll
       for (int e = 0; e < S::WIDTH; e++) {
@@ -211,40 +260,42 @@ struct Parameters {
         tb[e] = beta[j * S::WIDTH + e];
       }
     } else {
-      load_step<VEC ? FOUR : ONE>(tg, g, S::first(j));
-      load_step<VEC ? FOUR : ONE>(tb, b, S::first(j));
+      const uint32_t first = S::first(j);
+      load_step<ACCESS>(tg, g, load_at<ACCESS>(first, N));
+      load_step<ACCESS>(tb, b, load_at<ACCESS>(first, N));
+      settle<ACCESS>(tg, first, N);
+      settle<ACCESS>(tb, first, N);
     }
   }
 };
 
 // gamma * xhat + beta and the function, from x in registers
 template <int L, int E, int ACCESS>
-__device__ __forceinline__ void normalise(int func, float *out, const float (&x)[E], float mean, float ivar, const Parameters<L, E, ACCESS != ONE> &held, const float *gamma,
+__device__ __forceinline__ void normalise(int func, float *out, const float (&x)[E], float mean, float ivar, const Parameters<L, E, kept(ACCESS)> &held, const float *gamma,
                                           const float *beta, uint32_t N) {
-  using S = Share<L, E, ACCESS != ONE>;
+  using S = Share<L, E, ACCESS>;
 #pragma unroll
   for (int j = 0; j < S::STEPS; j++) {
     if (S::first(j) >= N) continue;
     float g[S::WIDTH], b[S::WIDTH], y[S::WIDTH];
-    held.step(gamma, beta, j, g, b);
+    held.step(gamma, beta, j, N, g, b);
 #pragma unroll
     for (int e = 0; e < S::WIDTH; e++) y[e] = g[e] * ((x[j * S::WIDTH + e] - mean) * ivar) + b[e];
     apply<S::WIDTH>(func, y);
-    store_step<ACCESS>(out + S::first(j), y);
+    store_step<ACCESS>(out + S::first(j), y, N - S::first(j));
   }
 }
 
 // rows that fit the registers of L threads
 template <int L, int E, int ACCESS, bool PACK>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a) {
-  constexpr bool VEC = ACCESS != ONE;
-  using S = Share<L, E, VEC>;
+  using S = Share<L, E, ACCESS>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
   __shared__ float part[2][L / 64 + 1];
   const uint32_t want = a.first_row + blockIdx.x * PER_BLOCK + threadIdx.x / L, row = min(want, a.rows - 1);
   const bool mine = want < a.rows;
   float x[E];
-  Parameters<L, E, VEC> held;
+  Parameters<L, E, kept(ACCESS)> held;
   S::template load<ACCESS>(x, a.in + (size_t)row * a.N, a.N);
   // the parameters are under way with the row where a wavefront or less holds it (12000 x 1024 20.6 -> 19.8 us, 60000 x 128 11.7 -> 10.6); more
   // threads per row lose more from the registers (2000 x 16384 55.3 -> 63.8)
@@ -257,7 +308,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a
     const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N;
 #pragma unroll
     for (int j = 0; j < S::STEPS; j++)
-      if (mine) pack_step(a.packed, w, e0 + S::first(j), S::first(j) < a.N, x + j * S::WIDTH);
+      if (mine) pack_step(a.packed, w, e0 + S::first(j), (int)a.N - (int)S::first(j), x + j * S::WIDTH);
   }
   float s = 0.f;
 #pragma unroll
@@ -268,7 +319,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a
   for (int j = 0; j < S::STEPS; j++)
 #pragma unroll
     for (int e = 0; e < S::WIDTH; e++) {
-      const float d = S::first(j) < a.N ? x[j * S::WIDTH + e] - mean : 0.f;
+      const float d = S::inside(j, e, a.N) ? x[j * S::WIDTH + e] - mean : 0.f;
       s += d * d;
     }
   const float ivar = 1.f / sqrtf(row_sum<L>(s, part[1]) / (float)a.N + a.eps);
@@ -283,9 +334,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_forward_kernel(Forward a
 
 // longer rows: pieces of PIECE values, one block each.  First the mean and the sum of squared deviations of every piece ...
 constexpr uint32_t PIECE = 4096;
-template <bool VEC, bool PACK>
+template <int ACCESS, bool PACK>
 __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *stats, uint32_t pieces) {
-  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  using S = Share<THREADS, PIECE / THREADS, ACCESS>;
   __shared__ float part[2][THREADS / 64];
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE);
   float x[PIECE / THREADS];
@@ -293,7 +344,7 @@ __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *s
   if (PACK) {
     const uint32_t w = a.per_sample == 1 ? row : row / a.per_sample, e0 = (row - w * a.per_sample) * a.N + piece * PIECE;
 #pragma unroll
-    for (int j = 0; j < S::STEPS; j++) pack_step(a.packed, w, e0 + S::first(j), S::first(j) < n, x + j * S::WIDTH);
+    for (int j = 0; j < S::STEPS; j++) pack_step(a.packed, w, e0 + S::first(j), (int)n - (int)S::first(j), x + j * S::WIDTH);
   }
   float s = 0.f;
 #pragma unroll
@@ -304,7 +355,7 @@ __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *s
   for (int j = 0; j < S::STEPS; j++)
 #pragma unroll
     for (int e = 0; e < S::WIDTH; e++) {
-      const float d = S::first(j) < n ? x[j * S::WIDTH + e] - mean : 0.f;
+      const float d = S::inside(j, e, n) ? x[j * S::WIDTH + e] - mean : 0.f;
       s += d * d;
     }
   s = row_sum<THREADS>(s, part[1]);
@@ -314,8 +365,7 @@ __global__ __launch_bounds__(THREADS) void ln_pieces_kernel(Forward a, float2 *s
 // n * (its mean - the row's mean)^2) and normalises its own piece
 template <int ACCESS>
 __global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const float2 *stats, uint32_t pieces) {
-  constexpr bool VEC = ACCESS != ONE;
-  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  using S = Share<THREADS, PIECE / THREADS, ACCESS>;
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, lane = threadIdx.x % 64, n = min(PIECE, a.N - piece * PIECE);
   const size_t at = (size_t)row * a.N + (size_t)piece * PIECE;
   float x[PIECE / THREADS];
@@ -332,7 +382,7 @@ __global__ __launch_bounds__(THREADS) void ln_apply_kernel(Forward a, const floa
   }
   const float ivar = 1.f / sqrtf(mt::over_lanes<mt::Sum, 64>(s) / (float)a.N + a.eps);
   const float *gamma = a.gamma + (size_t)piece * PIECE, *beta = a.beta + (size_t)piece * PIECE;
-  Parameters<THREADS, PIECE / THREADS, VEC> held;
+  Parameters<THREADS, PIECE / THREADS, kept(ACCESS)> held;
   held.load(gamma, beta, n);
   normalise<THREADS, PIECE / THREADS, ACCESS>(a.func, a.out + at, x, mean, ivar, held, gamma, beta, n);
   if (piece == 0 && threadIdx.x == 0) {
@@ -413,7 +463,7 @@ __global__ __launch_bounds__(SLICES == 1 ? THREADS : JOIN_COLUMNS * SLICES) void
 template <int L, int E, int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
   constexpr bool VEC = ACCESS != ONE;
-  using S = Share<L, E, VEC>;
+  using S = Share<L, E, ACCESS>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
   constexpr int W = S::WIDTH;
   __shared__ float part[2][2][L / 64 + 1];
@@ -443,7 +493,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     const auto in = rows.row(row);
     S::template load<ACCESS>(gr, a.delta + (size_t)row * a.N, a.N);
 #pragma unroll
-    for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(r[j], min(S::first(j), a.N - W));
+    for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(r[j], Rows::template at<ACCESS>(S::first(j), a.N));
   };
   if constexpr (EARLY) load(min(blockIdx.x * PER_BLOCK + sub, a.rows - 1), raw, g, &mean, &ivar);
   for (uint32_t first = blockIdx.x * PER_BLOCK; first < a.rows; first += stride, turn ^= 1u) {
@@ -457,7 +507,10 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     if constexpr (!HELD) load_parameters();
     __builtin_amdgcn_sched_barrier(0);  // all loads before the first use of one
 #pragma unroll
-    for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
+    for (int j = 0; j < S::STEPS; j++) {
+      raw[j].values(x + j * W);
+      Rows::template settle_values<ACCESS>(x + j * W, S::first(j), a.N);
+    }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
@@ -504,7 +557,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
         float t[W];
 #pragma unroll
         for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
-        store_step<ACCESS>(error + S::first(j), t);
+        store_step<ACCESS>(error + S::first(j), t, a.N - S::first(j));
       }
     }
     if constexpr (EARLY) {
@@ -521,8 +574,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 #pragma unroll
     for (int j = 0; j < S::STEPS; j++)
       if (S::first(j) < a.N) {
-        store_step<VEC ? FOUR : ONE>(pg + S::first(j), dg + j * W);
-        store_step<VEC ? FOUR : ONE>(pb + S::first(j), db + j * W);
+        store_step<kept(ACCESS)>(pg + S::first(j), dg + j * W, a.N - S::first(j));
+        store_step<kept(ACCESS)>(pb + S::first(j), db + j * W, a.N - S::first(j));
       }
     return;
   }
@@ -554,7 +607,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 template <int L, int E, int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Backward a, Rows rows, uint32_t first_row, uint32_t error_blocks) {
   constexpr bool VEC = ACCESS != ONE;
-  using S = Share<L, E, VEC>;
+  using S = Share<L, E, ACCESS>;
   constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1, BLOCK = L < 256 ? 256 : L;
   constexpr int W = S::WIDTH;
   if (blockIdx.x >= error_blocks) {
@@ -611,12 +664,15 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
   float x[E], g[E], gamma[E], beta[FUNC ? E : 1];
   S::template load<ACCESS>(g, a.delta + (size_t)row * a.N, a.N);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(raw[j], min(S::first(j), a.N - W));
+  for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(raw[j], Rows::template at<ACCESS>(S::first(j), a.N));
   S::load(gamma, a.gamma, a.N);
   if constexpr (FUNC) S::load(beta, a.beta, a.N);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
+  for (int j = 0; j < S::STEPS; j++) {
+    raw[j].values(x + j * W);
+    Rows::template settle_values<ACCESS>(x + j * W, S::first(j), a.N);
+  }
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int k = 0; k < E; k++) x[k] = (x[k] - mean) * ivar;
@@ -640,14 +696,15 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_few_kernel(Back
     float t[W];
 #pragma unroll
     for (int e = 0; e < W; e++) t[e] = ivar * ((g[j * W + e] - s1) - x[j * W + e] * s2);
-    store_step<ACCESS>(a.error + (size_t)row * a.N + S::first(j), t);
+    store_step<ACCESS>(a.error + (size_t)row * a.N + S::first(j), t, a.N - S::first(j));
   }
 }
 
 // longer rows: the two sums of every piece ...
-template <bool VEC, bool FUNC, class Rows>
+template <int ACCESS, bool FUNC, class Rows>
 __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a, Rows rows, float2 *sums, uint32_t pieces) {
-  using S = Share<THREADS, PIECE / THREADS, VEC>;
+  constexpr bool VEC = ACCESS != ONE;
+  using S = Share<THREADS, PIECE / THREADS, ACCESS>;
   constexpr int W = S::WIDTH;
   __shared__ float part[2][THREADS / 64];
   const uint32_t row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, n = min(PIECE, a.N - piece * PIECE), at = piece * PIECE;
@@ -657,13 +714,16 @@ __global__ __launch_bounds__(THREADS) void ln_backward_pieces_kernel(Backward a,
   float x[PIECE / THREADS], g[PIECE / THREADS];
   S::load(g, a.delta + (size_t)row * a.N + at, n);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) in.template load<VEC ? FOUR : ONE>(raw[j], at + min(S::first(j), n - W));
+  for (int j = 0; j < S::STEPS; j++) in.template load<ACCESS>(raw[j], (int)at + Rows::template at<ACCESS>(S::first(j), n));
   float gamma[PIECE / THREADS], beta[FUNC ? PIECE / THREADS : 1];
   S::load(gamma, a.gamma + at, n);
   if constexpr (FUNC) S::load(beta, a.beta + at, n);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int j = 0; j < S::STEPS; j++) raw[j].values(x + j * W);
+  for (int j = 0; j < S::STEPS; j++) {
+    raw[j].values(x + j * W);
+    Rows::template settle_values<ACCESS>(x + j * W, S::first(j), n);
+  }
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int k = 0; k < (int)(PIECE / THREADS); k++) x[k] = (x[k] - mean) * ivar;
@@ -693,7 +753,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
   __shared__ float4 terms[GROUP_ROWS];  // of each row: mean, ivar, sum(u) / N, sum(u * xhat) / N
   __shared__ float shares[2][SLICES][W][64];
   const uint32_t lane = threadIdx.x % 64, slice = threadIdx.x / 64;
-  const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * 64 + lane) * W, at = min(column, a.N - W);
+  const uint32_t group = blockIdx.x % groups, column = (blockIdx.x / groups * 64 + lane) * W;
+  const int at = load_at<ACCESS>(column, a.N), input_at = Rows::template at<ACCESS>(column, a.N);
   const uint32_t first = group * per_group, count = min(per_group, a.rows - first);
   // four rows at a time, the next four loaded before the first of them is stored (the error may be written over delta: each row of a
   // column is read and written by one thread)
@@ -704,13 +765,17 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
     for (uint32_t u = 0; u < AT_ONCE; u++) {
       const uint32_t row = first + min(k0 + u * SLICES, count - 1);
       load_step<ACCESS>(d[u], a.delta + (size_t)row * a.N, at);
-      rows.row(row).template load<ACCESS>(r[u], at);
+      rows.row(row).template load<ACCESS>(r[u], input_at);
     }
   };
   load(slice, raw, g);
   float gamma[W], beta[W], dg[W] = {}, db[W] = {};
-  load_step<VEC ? FOUR : ONE>(gamma, a.gamma, at);
-  if (FUNC) load_step<VEC ? FOUR : ONE>(beta, a.beta, at);
+  load_step<kept(ACCESS)>(gamma, a.gamma, at);
+  settle<ACCESS>(gamma, column, a.N);
+  if (FUNC) {
+    load_step<kept(ACCESS)>(beta, a.beta, at);
+    settle<ACCESS>(beta, column, a.N);
+  }
   // eight lanes per row, eight loads each under way
   for (uint32_t k = threadIdx.x / 8; k < count; k += THREADS / 8) {
     const float2 *p = sums + (size_t)(first + k) * pieces;
@@ -740,6 +805,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
       const float4 c = terms[k];
       float x[W], t[W];
       raw[u].values(x);
+      Rows::template settle_values<ACCESS>(x, column, a.N);
+      settle<ACCESS>(g[u], column, a.N);
 #pragma unroll
       for (uint32_t e = 0; e < W; e++) x[e] = (x[e] - c.x) * c.y;
       if constexpr (FUNC) fronts<W>(a.func, g[u], gamma, x, beta);
@@ -749,7 +816,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
         db[e] += g[u][e];
         t[e] = c.y * ((g[u][e] * gamma[e] - c.z) - x[e] * c.w);
       }
-      if (column < a.N) store_step<ACCESS>(a.error + (size_t)(first + k) * a.N + column, t);
+      if (column < a.N) store_step<ACCESS>(a.error + (size_t)(first + k) * a.N + column, t, a.N - column);
     }
 #pragma unroll
     for (uint32_t u = 0; u < AT_ONCE; u++) {
@@ -773,7 +840,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
     float s = 0.f;
 #pragma unroll
     for (uint32_t k = 0; k < SLICES; k++) s += shares[slice][k][e][lane];
-    out[column + e] = a.accumulate && groups == 1 ? out[column + e] + s : s;
+    if (ACCESS != FOUR_ANY || column + e < a.N) out[column + e] = a.accumulate && groups == 1 ? out[column + e] + s : s;
   }
 }
 
@@ -831,13 +898,32 @@ int geometry(const char *name, const mt_tensor *in, const mt_tensor *gamma, Geom
 bool same_sizes(const mt_tensor *a, const mt_tensor *b) { return mt::same_zyx(a, b) && a->w == b->w; }
 bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { return t->w == in->w && t->z == g.kept_z && t->y == g.kept_y && t->x == 1; }
 
-// rows of up to this many values are held in registers.  In the backward pass 1024 threads have room for 16 values each and their
-// share of two sums, but not for a function's parameters or an address per value too: 2000 x 16384 with tangence 134 us against 114 in
-// pieces, 2000 x 16383 185 against 129
+// rows of up to this many values are held in registers.  In the backward pass 1024 threads have room for 16 values each and their share
+// of two sums, but not for a function's parameters too (2000 x 16384 with tangence 134 us against 114 in pieces).  In fours from any address
+// they have it from fp32 input and pay for it with many rows (2000 x 16383 110 against 136, but 600 x 10319 34 against 27; from 8 bits
+// 1344 x 10319 62 against 48)
 constexpr uint32_t FORWARD_ROW = 32768, BACKWARD_ROW = 16384, BACKWARD_ROW_TIGHT = 8192;
 
 // blocks of one launch, at most: a grid has fewer than 2^32 threads
 constexpr uint32_t MOST_BLOCKS = 1u << 21;
+
+// calls f with how a kernel accesses the tensors
+template <class F>
+void with_access(int access, F &&f) {
+  if (access == FOUR_PAST)
+    f(std::integral_constant<int, FOUR_PAST>{});
+  else if (access == FOUR)
+    f(std::integral_constant<int, FOUR>{});
+  else if (access == FOUR_ANY)
+    f(std::integral_constant<int, FOUR_ANY>{});
+  else
+    f(std::integral_constant<int, ONE>{});
+}
+// Four values per access where rows are a multiple of four from 16-byte boundaries (`whole`), and from any address in rows of more than a
+// wavefront (1344 x 10319 backward 73 -> 59 us, 2000 x 16383 152 -> 111, 4000 x 4001 forward with 8 bits 47 -> 34).  Shorter rows have
+// more ends to take apart than accesses to save (30000 x 333 forward 14.2 us singly, 17.4 in fours)
+constexpr uint32_t ANY_ROW = 1024;
+int access_of(bool whole, uint32_t N, uint64_t bytes) { return whole ? mt::past_caches(bytes) ? FOUR_PAST : FOUR : N > ANY_ROW ? FOUR_ANY : ONE; }
 
 template <int L, int E>
 void forward_rows(Forward a, int access, bool pack) {
@@ -846,20 +932,15 @@ void forward_rows(Forward a, int access, bool pack) {
     const uint32_t left = a.rows - a.first_row, grid = cdiv(left, PER_BLOCK) < MOST_BLOCKS ? cdiv(left, PER_BLOCK) : MOST_BLOCKS;
     const auto go = [&](auto acc) {
       constexpr int ACCESS = decltype(acc)::value;
-      if constexpr (L >= 64 && ACCESS != ONE) {
+      if constexpr (L >= 64 && ACCESS != ONE) {  // (a group of 128 by 32 lanes)
         if (pack) {
           ln_forward_kernel<L, E, ACCESS, true><<<grid, BLOCK, 0, mt::stream()>>>(a);
           return;
         }
       }
-      ln_forward_kernel<L, E, ACCESS, false><<<grid, BLOCK, 0, mt::stream()>>>(a);
+      if constexpr (ACCESS != FOUR_ANY || L * E > (int)ANY_ROW) ln_forward_kernel<L, E, ACCESS, false><<<grid, BLOCK, 0, mt::stream()>>>(a);
     };
-    if (access == FOUR_PAST)
-      go(std::integral_constant<int, FOUR_PAST>{});
-    else if (access == FOUR)
-      go(std::integral_constant<int, FOUR>{});
-    else
-      go(std::integral_constant<int, ONE>{});
+    with_access(access, go);
     if (left <= grid * PER_BLOCK) return;
     a.first_row += grid * PER_BLOCK;
   }
@@ -884,18 +965,12 @@ int with_share(uint32_t N, F &&f) {
   return f(integral_constant<int, 1024>{}, integral_constant<int, 32>{});
 }
 
-// calls f with what a kernel is compiled for: how it accesses the tensors, whether a function stands behind the norm
+// calls f with that and whether a function stands behind the norm
 template <class F>
 void with_kind(int access, bool func, F &&f) {
-  const auto with_access = [&](auto acc) {
+  with_access(access, [&](auto acc) {
     if (func) f(acc, std::true_type{}); else f(acc, std::false_type{});
-  };
-  if (access == FOUR_PAST)
-    with_access(std::integral_constant<int, FOUR_PAST>{});
-  else if (access == FOUR)
-    with_access(std::integral_constant<int, FOUR>{});
-  else
-    with_access(std::integral_constant<int, ONE>{});
+  });
 }
 
 template <class Rows>
@@ -913,15 +988,17 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     a.func = MT_F_NONE;
   }
   const bool params = dgamma || dbeta;
-  const bool vec = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
+  const bool whole = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
   // (half of what the pass moves stands for the size of a tensor that is read and written: 4096 x 6144 62.6 -> 58.2 us)
-  const int access = !vec ? ONE : mt::past_caches(mt::count(delta) * (8 + Rows::BYTES) / 2) ? FOUR_PAST : FOUR;
+  const int access = x.in_fours() ? access_of(whole, g.N, mt::count(delta) * (8 + Rows::BYTES) / 2) : ONE;
+  const bool vec = access != ONE;
   // few rows: the parameter gradients beside the error instead of partial sums and their join
   const bool few = g.rows <= 512;
   uint32_t parts = 0;
   float *partial = nullptr;
   const bool beside = !params || few;  // no sums over rows in the error's threads
-  if (g.N <= (beside || (vec && a.func == MT_F_NONE) ? BACKWARD_ROW : BACKWARD_ROW_TIGHT)) {
+  const bool held = a.func == MT_F_NONE && (whole || (access == FOUR_ANY && Rows::BYTES == 4 && g.rows >= 1024));
+  if (g.N <= (beside || held ? BACKWARD_ROW : BACKWARD_ROW_TIGHT)) {
     int rc = with_share(g.N, [&](auto l, auto e) {
       constexpr int L = l, E = e;
       if constexpr (L * E <= (int)BACKWARD_ROW) {
@@ -930,7 +1007,9 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
           const auto go = [&](uint32_t first_row, uint32_t grid, uint32_t first_param_block) {
             with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
-              ln_backward_few_kernel<L, E, decltype(v)::value, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_row, first_param_block);
+              constexpr int ACCESS = decltype(v)::value;
+              if constexpr (ACCESS != FOUR_ANY || L * E > (int)ANY_ROW)
+                ln_backward_few_kernel<L, E, ACCESS, decltype(f)::value, Rows><<<grid, threads, 0, mt::stream()>>>(a, x, first_row, first_param_block);
             });
           };
           if (params && a.error != a.delta) {
@@ -955,7 +1034,8 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
           constexpr int ACCESS = decltype(v)::value;
           constexpr bool FUNC = decltype(f)::value;
-          if constexpr (L * E <= (int)BACKWARD_ROW_TIGHT || (ACCESS != ONE && !FUNC)) ln_backward_kernel<L, E, ACCESS, FUNC, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+          constexpr bool fits = L * E <= (int)BACKWARD_ROW_TIGHT || (!FUNC && (ACCESS == FOUR || ACCESS == FOUR_PAST || (ACCESS == FOUR_ANY && Rows::BYTES == 4)));
+          if constexpr (fits && (ACCESS != FOUR_ANY || L * E > (int)ANY_ROW)) ln_backward_kernel<L, E, ACCESS, FUNC, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
         });
       }
       return (int)MT_OK;
@@ -983,7 +1063,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
       constexpr int ACCESS = decltype(v)::value;
       constexpr bool FUNC = decltype(f)::value;
-      ln_backward_pieces_kernel<ACCESS != ONE, FUNC><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
+      ln_backward_pieces_kernel<kept(ACCESS), FUNC><<<g.rows * pieces, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces);
       ln_backward_columns_kernel<ACCESS, FUNC><<<groups * strips, THREADS, 0, mt::stream()>>>(a, x, piece_sums, pieces, groups, per_group, partial);
     });
     MT_LAUNCH_CHECK(name);
@@ -1066,10 +1146,12 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
   a.out = out->p; a.in = in->p; a.gamma = gamma->p; a.beta = beta->p; a.mean = mean ? mean->p : nullptr; a.ivar = ivar ? ivar->p : nullptr;
   a.packed = packed; a.rows = g.rows; a.N = g.N; a.per_sample = g.per_sample; a.eps = epsilon;
   a.func = func == MT_F_GELU ? MT_F_NONE : func;  // GeLU (double arithmetic, a library function) runs over the output afterwards
-  const bool vec = g.N % 4 == 0 && aligned16(a.out) && aligned16(a.in) && aligned16(a.gamma) && aligned16(a.beta);
-  const int access = !vec ? ONE : mt::past_caches(mt::count(in) * 4) ? FOUR_PAST : FOUR;
-  // the same pass can leave the 8 bits where a row starts at a group's first value and 32 lanes hold a group
-  const bool pack = packed_input && vec && g.N > 128 && (g.N % mt::PACK_GROUP == 0 || g.per_sample == 1);
+  const bool whole = g.N % 4 == 0 && aligned16(a.out) && aligned16(a.in) && aligned16(a.gamma) && aligned16(a.beta);
+  // the same pass can leave the 8 bits where a row starts at a group's first value and 32 lanes hold a group; it takes fours from any address
+  // then (12000 x 1001 33 us in two passes, 29 in one; 33 x 1001 7.2 and 4.6)
+  const bool pack = packed_input && g.N > 128 && (g.N % mt::PACK_GROUP == 0 || g.per_sample == 1);
+  int access = access_of(whole, g.N, mt::count(in) * 4);
+  if (pack && access == ONE) access = FOUR_ANY;
   if (packed_input && !pack && (rc = mt_pack(packed_input, in))) return rc;
   if (packed_input) mt::note_write(packed.q, mt::packed_bytes(packed));
   {
@@ -1087,14 +1169,15 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
       if ((rc = ln_workspace(2 * (size_t)g.rows * pieces, &ws))) return rc;
       float2 *stats = reinterpret_cast<float2 *>(ws);
       const unsigned grid = g.rows * pieces;
-      if (pack)
-        ln_pieces_kernel<true, true><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
-      else if (vec)
-        ln_pieces_kernel<true, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
-      else
-        ln_pieces_kernel<false, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      with_access(access == FOUR_PAST ? FOUR : access, [&](auto acc) {
+        constexpr int ACCESS = kept(decltype(acc)::value);
+        if (pack)
+          ln_pieces_kernel<ACCESS, true><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+        else
+          ln_pieces_kernel<ACCESS, false><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces);
+      });
       MT_LAUNCH_CHECK(name);
-      with_kind(access, false, [&](auto v, auto) { ln_apply_kernel<decltype(v)::value><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces); });
+      with_access(access, [&](auto acc) { ln_apply_kernel<decltype(acc)::value><<<grid, THREADS, 0, mt::stream()>>>(a, stats, pieces); });
       MT_LAUNCH_CHECK(name);
     }
   }

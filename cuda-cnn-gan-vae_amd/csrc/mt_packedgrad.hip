@@ -9,7 +9,8 @@
 //   exact; products below 2^-110 lose the bits that no normal bf16 number holds).
 //   Two fp16 numbers, rounded: the first off by at most 2^-12 of the product, the second by 2^-12 of that: 2^-24, the rounding of an
 //   fp32 product.  fp16 has little range: powers of two per row of dweight (of the largest delta) and per group (of the largest step)
-//   bring all products below 2^15, and small ones are off by 2^-25, nothing beside the rounding of the row's largest as long as
+//   bring all products below 2^15, and small ones are off by 2^-25 (fp16 keeps its subnormal numbers here, in the matrix
+//   instruction too), nothing beside the rounding of the row's largest as long as
 //   that is not small itself.  The block checks that, and starts again with three numbers where it is not so.  The powers need a
 //   look at all of delta before (a launch that reads it once and sums the columns for dbias on the way), so this is for products that
 //   are worth it.

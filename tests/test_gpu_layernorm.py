@@ -123,7 +123,8 @@ def test_geometries(mt, shape, pshape, shift, func):
 
 
 @pytest.mark.parametrize("rows,n,func", [(600, 8196, "tangence"), (257, 16388, None), (530, 8195, "sigmoid"), (17, 16385, None), (300, 20000, "relu"), (16, 49152, None),
-                                         (33, 49156, "tangence"), (520, 17001, None)])
+                                         (33, 49156, "tangence"), (520, 17001, None), (1030, 9001, None), (1024, 12291, None), (513, 12290, "sigmoid"),
+                                         (20, 36866, None), (9, 36867, "tangence"), (1027, 16383, None)])
 def test_many_long_rows(mt, rows, n, func):
     """Sums over rows that are cut into pieces: several groups of rows, groups of every size, error beside and over delta."""
     x, gamma, beta, delta = inputs(rows + n, (rows, 1, n, 1), (1, 1, n, 1))
@@ -314,7 +315,7 @@ def test_same_bits_every_time(mt, rows, n):
             assert all(np.array_equal(got[k], b[k]) for k in b)
 
 
-@pytest.mark.parametrize("n", [30, 1000, 4096, 40000])
+@pytest.mark.parametrize("n", [30, 333, 1000, 1025, 1026, 1027, 4096, 5003, 9001, 36866, 36867, 40000])
 def test_nothing_is_written_beside_the_results(mt, n):
     """Guard values in front of and behind every result stay."""
     shape, pshape = (5, 1, n, 1), (1, 1, n, 1)

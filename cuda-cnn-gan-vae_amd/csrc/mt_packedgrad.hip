@@ -9,15 +9,14 @@
 //   exact; products below 2^-110 lose the bits that no normal bf16 number holds).
 //   Two fp16 numbers, rounded: the first off by at most 2^-12 of the product, the second by 2^-12 of that: 2^-24, the rounding of an
 //   fp32 product.  fp16 has little range: powers of two per row of dweight (of the largest delta) and per group (of the largest step)
-//   bring all products below 2^15, and small ones are off by 2^-25 (fp16 keeps its subnormal numbers here, in the matrix
-//   instruction too), nothing beside the rounding of the row's largest as long as
-//   that is not small itself.  The block checks that, and starts again with three numbers where it is not so.  The powers need a
-//   look at all of delta before (a launch that reads it once and sums the columns for dbias on the way), so this is for products that
-//   are worth it.
+//   bring all products below 2^15, and small ones are off by 2^-25 (fp16 keeps its subnormal numbers here, in the matrix instruction
+//   too): nothing beside the rounding of the row's largest as long as that is not small itself.  The block checks that, and starts
+//   again with three numbers where it is not so.  The powers need a look at all of delta before (a launch that reads it once and sums
+//   the columns for dbias on the way), so this is for products that are worth it.
 // Three (two) 16-bit matrix instructions multiply what one fp32 product would, at a third (half) of a rate where the library's bf16
 // product reaches 1295 TFLOP/s; the fp32 matrix instructions reach 157 at most.  4096^3: 315 to 337 us in two numbers, 366 to 398 in
 // three (a chip that draws less power is faster: the clock falls to 1.9 GHz in these loops, and the matrix instructions of one wavefront
-// and the vector instructions of the other add up to 94 % of the cycles).  The second sum is one fp32 multiply-add per element of
+// and the vector instructions of the other add up to 92 % of the cycles).  The second sum is one fp32 multiply-add per element of
 // delta on the way.
 //
 // A column tile is one group, so that a sample has one (low, step) in it.  A block is four wavefronts, each with its own 32 or
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(Wgra
   __shared__ uintx4 cols[KW][2][KSTEP / 8][128];  // [eight samples][column]
   __shared__ float2 scale[KW][2][KSTEP];          // (step, low + 128 * step)
   __shared__ float4 offsets[4][TM][8];            // the second sum of every row of a wavefront
-  __shared__ int4 powers[HALVES ? 4 : 1][TM][8];    // the power of two that its products lack
+  __shared__ int4 powers[HALVES ? 4 : 1][TM][8];  // the power of two that its products lack
   __shared__ float halves[KW > 1 ? 2 : 1][4][TM][32];
   const uint32_t lane = threadIdx.x & 63u, r = lane & 31u, half = lane >> 5;
   const uint32_t kw = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u % 4u);
@@ -355,7 +354,10 @@ __global__ __launch_bounds__(THREADS * KW, 2 / KW) void packed_wgrad_kernel(Wgra
     __syncthreads();
     bool good = true;
 #pragma unroll
-    for (int m = 0; m < TM; m++) good = good && (most[m] == 0.f || most_step == 0.f || ((seen[0][wave][m][r] | seen[KW - 1][wave][m][r]) & 0x40004000u) != 0u);
+    for (int m = 0; m < TM; m++) {
+      const bool large = ((seen[0][wave][m][r] | seen[KW - 1][wave][m][r]) & 0x40004000u) != 0u;
+      good = good && (large || m0 + r * TM + m >= a.Out || most[m] == 0.f || most_step == 0.f);
+    }
     if (!__syncthreads_and(good)) {
       clear();
 #pragma unroll

@@ -183,6 +183,25 @@ def test_linear_unequal_magnitudes(mt, b, n_in, n_out, what):
     assert np.array_equal(added[0], dw + np.float32(1)) and np.array_equal(added[1], db + np.float32(1))
 
 
+@pytest.mark.parametrize("shift", [1, 2, 3])
+@pytest.mark.parametrize("b,n_in,n_out", [(40, 300, 140), (300, 260, 128), (1500, 2000, 1500)])
+def test_linear_off_a_16_byte_boundary(mt, b, n_in, n_out, shift):
+    """delta, dweight and dbias `shift` floats behind a 16-byte boundary: the same bits, nothing written beside them."""
+    x, delta = Nrm(1, b, 1, n_in, 1), Nrm(2, b, 1, n_out, 1)
+    want = run_linear(mt, x, delta)
+    pk = mt.CPackedTensor(*x.shape)
+    mt.CTensorMath.Pack(pk, up(mt, x))
+    held = []
+    for a, shape in ((delta, delta.shape), (None, (1, 1, n_out, n_in)), (None, (1, 1, n_out, 1))):
+        n = int(np.prod(shape))
+        whole = up(mt, np.concatenate([np.full(shift, 9), np.full(n, 7) if a is None else a.ravel(), np.full(8, 9)]).reshape(1, 1, 1, -1))
+        held.append((whole, mt.CTensor.wrap(whole.ptr.value + 4 * shift, shape), n))
+    mt.Fused.LinearBackwardWeightsSum(held[1][1], held[2][1], pk, held[0][1], accumulate=False)
+    for (whole, _, n), w in zip(held[1:], want):
+        got = whole.numpy().ravel()
+        assert np.array_equal(got[shift:shift + n], w.ravel()) and (got[:shift] == 9).all() and (got[shift + n:] == 9).all()
+
+
 @pytest.mark.parametrize("b,n_in,n_out", [(5, 100, 30), (300, 257, 129), (4096, 128, 64), (64, 1024, 1024)])
 def test_linear_adds_and_repeats(mt, b, n_in, n_out):
     x, delta = Nrm(1, b, 1, n_in, 1), Nrm(2, b, n_out, 1, 1)      # delta seen as [B,Out,1,1]

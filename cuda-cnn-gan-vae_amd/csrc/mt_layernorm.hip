@@ -459,15 +459,20 @@ __global__ __launch_bounds__(SLICES == 1 ? THREADS : JOIN_COLUMNS * SLICES) void
   if (i < N) out[i] = accumulate ? out[i] + s : s;
 }
 
+// Threads of its block: two wavefronts per SIMD, whose sums are joined in LDS, where the registers of a row's loads leave room (256 threads:
+// 4000 x 4001 49 us against 45, from 8 bits 46 against 38, 6000 x 777 17.4 against 14.8); sixteen values per thread in fours from 16-byte
+// boundaries have enough under way with one (12000 x 1000 32.1 us, 34.1 with 512 threads)
+constexpr int backward_block(int L, int E, int access) { return L > 256 ? L : E == 16 && (access == FOUR || access == FOUR_PAST) ? 256 : 512; }
+
 // rows that fit the registers of L threads; a block walks over the rows and keeps its share of dgamma and dbeta in registers
 template <int L, int E, int ACCESS, bool FUNC, class Rows>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
+__global__ __launch_bounds__(backward_block(L, E, ACCESS)) void ln_backward_kernel(Backward a, Rows rows, float *partial) {
   constexpr bool VEC = ACCESS != ONE;
   using S = Share<L, E, ACCESS>;
-  constexpr uint32_t PER_BLOCK = L < 256 ? 256 / L : 1;
+  constexpr uint32_t BLOCK = backward_block(L, E, ACCESS), PER_BLOCK = BLOCK / L;
   constexpr int W = S::WIDTH;
-  __shared__ float part[2][2][L / 64 + 1];
-  __shared__ float shared[L < 256 ? 2 * 256 * E : 1];
+  __shared__ float part[2][2][PER_BLOCK][L / 64 + 1];
+  __shared__ float shared[PER_BLOCK > 1 ? 2 * BLOCK * E : 1];
   const uint32_t sub = threadIdx.x / L, lane = threadIdx.x % L;
   constexpr bool HELD = L < 1024;  // gamma and beta stay in registers; 1024 threads load them for every row
   float dg[E], db[E], gamma[E], beta[FUNC ? E : 1];
@@ -535,16 +540,16 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     s2 = mt::over_lanes<mt::Sum, L < 64 ? L : 64>(s2);
     if (L > 64) {
       if (threadIdx.x % 64 == 0) {
-        part[turn][0][threadIdx.x / 64] = s1;
-        part[turn][1][threadIdx.x / 64] = s2;
+        part[turn][0][sub][lane / 64] = s1;
+        part[turn][1][sub][lane / 64] = s2;
       }
       __syncthreads();
-      s1 = part[turn][0][0];
-      s2 = part[turn][1][0];
+      s1 = part[turn][0][sub][0];
+      s2 = part[turn][1][sub][0];
 #pragma unroll
       for (int k = 1; k < L / 64; k++) {
-        s1 += part[turn][0][k];
-        s2 += part[turn][1][k];
+        s1 += part[turn][0][sub][k];
+        s2 += part[turn][1][sub][k];
       }
     }
     s1 /= (float)a.N;
@@ -570,7 +575,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
     }
   }
   float *pg = partial + (size_t)blockIdx.x * a.N, *pb = partial + ((size_t)gridDim.x + blockIdx.x) * a.N;
-  if (L >= 256) {
+  if (PER_BLOCK == 1) {
 #pragma unroll
     for (int j = 0; j < S::STEPS; j++)
       if (S::first(j) < a.N) {
@@ -585,20 +590,19 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void ln_backward_kernel(Backward
 #pragma unroll
     for (int e = 0; e < W; e++) {
       shared[sub * (L * E) + S::first(j) + e] = dg[j * W + e];
-      shared[256 * E + sub * (L * E) + S::first(j) + e] = db[j * W + e];
+      shared[BLOCK * E + sub * (L * E) + S::first(j) + e] = db[j * W + e];
     }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < a.N; i += 256) {
+  for (uint32_t i = threadIdx.x; i < a.N; i += BLOCK) {
     float sg = 0.f, sb = 0.f;
 #pragma unroll
     for (uint32_t k = 0; k < PER_BLOCK; k++) {
       sg += shared[k * (L * E) + i];
-      sb += shared[256 * E + k * (L * E) + i];
+      sb += shared[BLOCK * E + k * (L * E) + i];
     }
     pg[i] = sg;
     pb[i] = sb;
   }
-  (void)lane;
 }
 
 // The error alone, one row per L threads, and beside it in the same launch (blocks from error_blocks on) dgamma and dbeta straight
@@ -1023,19 +1027,18 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
           }
           return (int)MT_OK;
         }
-        parts = cdiv(g.rows, per_block);
+        const int block = backward_block(L, E, access);
+        parts = cdiv(g.rows, block / L);
         // one block per compute unit: its next row is on the way while it sums, and more blocks mean more partial sums (4096 x 6144: 60.0 us
-        // with 256, 66.1 with 512, 74.7 with 1024; 1024 x 8192: 23.0, 30.6, 41.7).  Two where a thread holds few values or loads them
-        // singly and the rows are many (8192 x 2048 from 8 bits 35.4 us with 256, 29.9 with 512; 1024 x 2048 10.7, 12.9)
-        const uint32_t most = (E <= 8 || !vec) && parts >= 4096 ? 512 : 256;
-        if (parts > most) parts = most;
+        // with 256, 66.1 with 512, 74.7 with 1024; 1024 x 8192: 23.0, 30.6, 41.7)
+        if (parts > 256) parts = 256;
         int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
         if (rc) return rc;
         with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
           constexpr int ACCESS = decltype(v)::value;
           constexpr bool FUNC = decltype(f)::value;
           constexpr bool fits = L * E <= (int)BACKWARD_ROW_TIGHT || (!FUNC && (ACCESS == FOUR || ACCESS == FOUR_PAST || (ACCESS == FOUR_ANY && Rows::BYTES == 4)));
-          if constexpr (fits && (ACCESS != FOUR_ANY || L * E > (int)ANY_ROW)) ln_backward_kernel<L, E, ACCESS, FUNC, Rows><<<parts, threads, 0, mt::stream()>>>(a, x, partial);
+          if constexpr (fits && (ACCESS != FOUR_ANY || L * E > (int)ANY_ROW)) ln_backward_kernel<L, E, ACCESS, FUNC, Rows><<<parts, block, 0, mt::stream()>>>(a, x, partial);
         });
       }
       return (int)MT_OK;

@@ -401,8 +401,8 @@ int mt_convolution_backward_weights_sum(const mt_tensor *dkernel, int32_t dkerne
  * an order that depends on the sizes and on whether the tensors are 16-byte aligned: the same call gives the same bits.
  * A NaN or an infinity in a row makes that row of xhat NaN, and with it the row's error and the dgamma it adds to (what func
  * makes of a NaN is its own: MT_F_RELU makes it 0).  Values whose squared deviations overflow (1.8e19 from their mean) have an
- * ivar of 0.  At most 2^31 - 1 rows, of at most 2^31 - 17 values, and fewer than 2^36 values in all where the rows are longer
- * than 8192.
+ * ivar of 0.  At most 2^31 - 1 rows, of at most 2^31 - 17 values; the backward pass takes fewer than 2^36 values in
+ * all where the rows are longer than 8192.
  * No result may share memory with another tensor, but for the two cases named below.
  *
  * mt_layernorm_forward_func: mean and ivar (NULL to skip) are what the backward pass needs.  output may be the same tensor as

@@ -160,6 +160,30 @@ def test_past_the_caches(mt, rows, n, func):
     assert all(np.array_equal(results[0][k], results[0][k + 3]) for k in (4, 5, 6, 10, 11, 12))
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_long_rows_beyond_the_caches(mt, packed):
+    """Rows in pieces, more of them than the caches hold: some at a time.  Every row as it would be alone."""
+    n, rows = 40001, 2000
+    x = mt.CTensor(rows, 1, n, 1)
+    mt.CTensorMath.SetNormalNoise(x, 3)
+    gamma, beta = up(mt, Nrm(1, 1, 1, n, 1)), up(mt, Nrm(2, 1, 1, n, 1))
+    out, mean, ivar, pk = mt.CTensor(rows, 1, n, 1), mt.CTensor(rows, 1, 1, 1), mt.CTensor(rows, 1, 1, 1), mt.CPackedTensor(rows, 1, n, 1) if packed else None
+    mt.Fused.LayerNormForward(out, x, gamma, beta, mean, ivar, pk, 1e-6, "tangence")
+    m, v = mean.numpy().ravel(), ivar.numpy().ravel()
+    values = mt.CTensor(rows, 1, n, 1)
+    if packed:
+        mt.CTensorMath.Unpack(values, pk)
+    for row in (0, 1, 1046, 1047, 1048, 1049, 1999):   # around the rows at which a part of 160 MiB ends
+        one = mt.CTensor.wrap(x.ptr.value + 4 * n * row, (1, 1, n, 1))
+        o1, m1, v1, p1 = mt.CTensor(1, 1, n, 1), mt.CTensor(1, 1, 1, 1), mt.CTensor(1, 1, 1, 1), mt.CPackedTensor(1, 1, n, 1)
+        mt.Fused.LayerNormForward(o1, one, gamma, beta, m1, v1, p1 if packed else None, 1e-6, "tangence")
+        assert np.array_equal(mt.CTensor.wrap(out.ptr.value + 4 * n * row, (1, 1, n, 1)).numpy(), o1.numpy())
+        assert m[row] == m1.numpy().item() and v[row] == v1.numpy().item()
+        if packed:
+            mt.CTensorMath.Unpack(o1, p1)
+            assert np.array_equal(mt.CTensor.wrap(values.ptr.value + 4 * n * row, (1, 1, n, 1)).numpy(), o1.numpy())
+
+
 def test_squares_that_overflow(mt):
     """Deviations above 1.8e19: no variance that fp32 holds, the row counts as having none of its values apart."""
     for n in (100, 1024, 4096, 40000):

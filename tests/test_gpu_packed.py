@@ -325,9 +325,10 @@ def test_a_training_step(mt, b, n_in, n_hidden, n_out):
         assert np.linalg.norm(got[key].reshape(want.shape) - want) <= 0.05 * np.linalg.norm(want), key
 
 
-def test_a_recorded_step_replays(mt):
+@pytest.mark.parametrize("b,n_in,n_hidden,n_out", [(130, 700, 1024, 90), (1500, 2000, 2001, 1500)])
+def test_a_recorded_step_replays(mt, b, n_in, n_hidden, n_out):
     """Recorded once, replayed with new inputs, with eager work of other sizes on the same workspaces between the replays."""
-    _, x, _, t, step = make_step(mt, 130, 700, 1024, 90)
+    _, x, _, t, step = make_step(mt, b, n_in, n_hidden, n_out)
     other = make_step(mt, 77, 300, 2500, 33, seed=40)[4]
     step()
     other()

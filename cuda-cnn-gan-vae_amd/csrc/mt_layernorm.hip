@@ -848,8 +848,19 @@ __global__ __launch_bounds__(THREADS) void ln_backward_columns_kernel(Backward a
   }
 }
 
-// error = delta * f'(gamma * xhat + beta) alone, for a function that the kernels above do not hold (GeLU: double arithmetic and two
-// library functions); the backward pass then starts from it
+// The derivative of what the forward pass computes for GeLU, v * s(v) with s(v) = 1 / (1 + exp(-2 u)) and u = sqrt(2 / pi) * (v + 0.044715 * v^3):
+//   s + 2 * v * s * (1 - s) * u'
+// with e = exp(-2 |u|), s * (1 - s) = e / (1 + e)^2: no difference of neighbouring numbers.  (Not MT_F_DIFFERENTIAL + MT_F_GELU: that is the
+// function layer's formula, as the reference's layer trains with it, and up to three quarters away from the slope.)
+__device__ __forceinline__ float gelu_slope(float v) {
+  const float a = sqrtf(2.f / 3.141592654f), u = a * (v + 0.044715f * (v * v * v)), size = fabsf(u);
+  const float e = expf(-2.f * size), r = mt::reciprocal(1.f + e), s = u < 0.f ? e * r : r;
+  // (beyond 40 the product is below 1e-30, but an infinite cube would make it a NaN; a NaN stays one in s)
+  return size < 40.f ? s + 2.f * v * (e * r * r) * (a * (1.f + 0.134145f * (v * v))) : s;
+}
+
+// error = delta * f'(gamma * xhat + beta) alone, for GeLU, whose exponential and polynomial the kernels above do not hold; the backward
+// pass then starts from it
 template <class Rows>
 __global__ __launch_bounds__(THREADS) void ln_front_kernel(Backward a, Rows rows) {
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -861,7 +872,7 @@ __global__ __launch_bounds__(THREADS) void ln_front_kernel(Backward a, Rows rows
       in.template load<ONE>(raw, i);
       raw.values(&x);
       const size_t e = (size_t)row * a.N + i;
-      a.error[e] = a.delta[e] * mt::apply_func(MT_F_DIFFERENTIAL + a.func, a.gamma[i] * ((x - mean) * ivar) + a.beta[i]);
+      a.error[e] = a.delta[e] * gelu_slope(a.gamma[i] * ((x - mean) * ivar) + a.beta[i]);
     }
   }
 }

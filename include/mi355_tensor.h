@@ -411,7 +411,8 @@ int mt_convolution_backward_weights_sum(const mt_tensor *dkernel, int32_t dkerne
 int mt_layernorm_forward_func(const mt_tensor *output, const mt_tensor *input, const mt_tensor *gamma, const mt_tensor *beta, const mt_tensor *mean,
                               const mt_tensor *ivar, const mt_packed_tensor *packed_input, float epsilon, int func);
 /* The backward pass (no counterpart in the reference).  delta: the gradient of func(gamma*xhat + beta); with
- * g = delta*func'(gamma*xhat + beta) and u = g*gamma
+ * g = delta*func'(gamma*xhat + beta) and u = g*gamma  (func' the derivative of what the forward pass computes; for MT_F_GELU that is not the
+ * formula of MT_F_DIFFERENTIAL + MT_F_GELU, which the function layer keeps from the reference and which is no derivative of MT_F_GELU)
  *   error = ivar*(u - sum(u)/N - xhat*sum(u*xhat)/N) over each row, dgamma = sum over the rows of g*xhat, dbeta of g.
  * accumulate: 1 adds the two sums to what dgamma and dbeta (sizes of gamma, NULL to skip) hold, as the other backward entry
  * points do; 0 overwrites it.  input, mean, ivar: as the forward pass read and left them.  beta is needed unless func is

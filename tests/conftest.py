@@ -19,6 +19,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
 
 
+# Tests that expect a value which is wrong, with the reason.  They run as they are and have to fail.
+WRONG_EXPECTATIONS = {
+    "test_gpu_layernorm.py::test_functions[%d-gelu]" % n:
+        "takes the function layer's formula for GeLU's slope, which is not the derivative of GeLU (0.399 at 0, where it is 0.5); "
+        "test_gpu_layernorm_edges.py holds the gradient against float64 and against differences"
+    for n in (60, 1001, 2048, 20000, 40000)}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        reason = WRONG_EXPECTATIONS.get("%s::%s" % (os.path.basename(str(item.fspath)), item.name))
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, raises=AssertionError, strict=True))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     if not oracle_api.available("oracle"):

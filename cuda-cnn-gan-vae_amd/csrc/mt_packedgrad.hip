@@ -13,8 +13,10 @@
 // whose products with q - zero the matrix cores add up in fp32, in one of two ways.
 //   Three bf16 numbers: its upper 8 significant bits, the next 8, the last 8 (cutting instead of rounding makes every remainder
 //   exact; products below 2^-110 lose the bits that no normal bf16 number holds).
-//   Two fp16 numbers, rounded: the first off by at most 2^-12 of the product, the second by 2^-12 of that: 2^-24, the rounding of an
-//   fp32 product.  fp16 has little range: powers of two per row of dweight (of the largest delta) and per group (of the largest step)
+//   Two fp16 numbers, rounded: the first (11 significant bits) off by at most 2^-11 of the product, the second by 2^-12 of what is left:
+//   2^-23 of the product at most, twice the rounding of an fp32 product (root mean square over all mantissas 3.7e-8, of fp32 2.4e-8).  That is
+//   a bit less than the three numbers hold, for two thirds of the matrix instructions; sums of thousands of such products carry fp32
+//   roundings of that size anyway.  fp16 has little range: powers of two per row of dweight (of the largest delta) and per group (of the largest step)
 //   bring all products below 2^15, and small ones are off by 2^-25 (fp16 keeps its subnormal numbers here, in the matrix instruction
 //   too): nothing beside the rounding of the row's largest as long as that is not small itself.  The block checks that, and starts
 //   again with three numbers where it is not so.  The powers need a look at all of delta before (a launch that reads it once and sums

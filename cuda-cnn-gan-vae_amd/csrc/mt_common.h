@@ -28,6 +28,7 @@ int set_walk_fair(int v);
 int set_igemm_fair(int v);
 int set_first_layer(int v);   // forward convolutions of 3-channel images on the input-patch kernel: 0 never, 1 wherever the shape allows
 int set_nontemporal(int v);   // streaming kernels read and write past the caches: 0 never, 1 always, 2 tensors of 128 MiB and more
+int set_linear_packed(int v);  // variant and parts of mt_linear_backward_weights_sum_packed (0: choose)
 bool past_caches(size_t bytes);  // does that option send a tensor of so many bytes past the caches
 int set_image_strip(int v);   // rows per strip of the image layer's product kernel on 64-column images (0: choose)
 int set_conv_patch(int v);     // 3x3 stride-1 forward convolutions from at most 32 channels on large images from patches in LDS: 1 (default) / 0 never / n: from n filters on

@@ -531,8 +531,16 @@ struct Plan {
   uint32_t rows, split;
   bool pair, half;
 };
+int g_linear_packed = 0;  // option "linear_packed": 0 choose, else variant 1 ... 5 and ten times the parts of the batch
+constexpr uint32_t MOST_PARTS = 128;
 Plan choose(uint32_t Out, uint32_t groups, uint32_t samples, size_t n) {
   const uint32_t steps = cdiv(samples, KSTEP);
+  if (g_linear_packed != 0) {
+    const int variant = g_linear_packed % 10;
+    const bool wide = (variant == 3 || variant == 5) && Out % 2 == 0;
+    const uint32_t parts = g_linear_packed / 10 ? g_linear_packed / 10 : 1;
+    return Plan{wide ? 256u : 128u, n >= (1u << 29) ? 1 : parts < steps ? parts : steps, variant != 1 && !wide, variant >= 4};
+  }
   const double look = 4.0 + (double)samples * Out * 4 / 5.6e6;  // what the launch before and its results cost
   Plan best{128, 1, false, false};
   double least = 1e30;
@@ -542,7 +550,7 @@ Plan choose(uint32_t Out, uint32_t groups, uint32_t samples, size_t n) {
     if (rows == 256 && Out % 2 != 0) continue;  // rows are loaded in pairs there, which must not straddle the end
     const double fixed = kind == 0 ? 5.0 : kind == 1 ? 6.0 : 6.5, one = kind == 0 ? 1.75 : kind == 1 ? 3.0 : 2.8, two = kind == 0 ? 3.25 : kind == 1 ? 6.0 : 5.7;
     const size_t tiles = (size_t)cdiv(Out, rows) * groups;
-    for (uint32_t split = 1; split <= 128 && split <= steps; split += split < 4 ? 1 : split / 2) {
+    for (uint32_t split = 1; split <= MOST_PARTS && split <= steps; split += split < 4 ? 1 : split / 2) {
       if (split > 1 && n >= (1u << 29)) break;  // a join is one launch of fewer than 2^32 threads
       const size_t blocks = tiles * split;
       const size_t rest = blocks % 512;
@@ -561,6 +569,16 @@ Plan choose(uint32_t Out, uint32_t groups, uint32_t samples, size_t n) {
 }
 
 }  // namespace
+
+namespace mt {
+int set_linear_packed(int v) {
+  const int variant = v % 10;
+  if (v < 0 || (v != 0 && (variant < 1 || variant > 5)) || v / 10 > (int)MOST_PARTS)
+    return fail(MT_E_ARGUMENT, "linear_packed must be 0 (choose) or a variant 1 to 5 plus ten times 0 to %u parts of the batch", MOST_PARTS);
+  g_linear_packed = v;
+  return MT_OK;
+}
+}  // namespace mt
 
 extern "C" {
 

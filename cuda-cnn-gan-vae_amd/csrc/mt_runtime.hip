@@ -299,6 +299,7 @@ int mt_set_option(const char *name, int value) {
   if (name && strcmp(name, "pack_refresh") == 0) return mt::set_pack_refresh(value);
   if (name && strcmp(name, "adam_vec") == 0) return mt::set_adam_vec(value);
   if (name && strcmp(name, "nontemporal") == 0) return mt::set_nontemporal(value);
+  if (name && strcmp(name, "linear_packed") == 0) return mt::set_linear_packed(value);
   if (name && strcmp(name, "image_strip") == 0) return mt::set_image_strip(value);
   if (name && strcmp(name, "first_layer") == 0) return mt::set_first_layer(value);
   if (name && strcmp(name, "walk_blocks") == 0) return mt::set_walk_blocks(value);

@@ -162,6 +162,9 @@ int mt_timer_destroy(void *timer);
  *                    2 (default) products per input pixel on the 16x16x4 matrix instruction where the shape allows /
  *                    1 the 4x4x1 matrix instruction where the shape allows / 0 the vector ALUs
  *   "image_strip"    rows per strip of the image layer's product kernel on images of 64 columns (0, default: 8 or 4)
+ *   "linear_packed"  0 (default) mt_linear_backward_weights_sum_packed chooses per shape / k + 10*s: variant k -- 1 128 rows of dweight per
+ *                    block, 2 the same with two groups of wavefronts, 3 256 rows (an even number of features, else 2), all in three
+ *                    bf16 numbers; 4 and 5 as 2 and 3 in two fp16 numbers -- and the batch in s parts (0: one; 128 at most)
  *   "nontemporal"    2 (default) the re-sampling, pooling, large-batch batch-norm, layer-norm and 8-bit packing kernels read and
  *                    write tensors of 128 MiB and more past the caches (each element is touched once) / 1 always / 0 never
  *   "staged_uploads" 1 (default) mt_copy_h2d of at most 64 KiB copies the caller's buffer into a pinned slot at once and queues

@@ -8,6 +8,7 @@
 // error.  A row is therefore held in registers between its sums and its results wherever it fits (one to 1024 threads per row, up
 // to 32 values per thread); longer rows are cut into pieces that several blocks share, and their second look at x finds it in
 // the caches.  Variances are sums of squared deviations from the mean (two passes over registers), never E[x^2] - E[x]^2.
+#include <initializer_list>
 #include <type_traits>
 
 #include "mt_packed.h"
@@ -911,6 +912,12 @@ int geometry(const char *name, const mt_tensor *in, const mt_tensor *gamma, Geom
   return MT_OK;
 }
 bool same_sizes(const mt_tensor *a, const mt_tensor *b) { return mt::same_zyx(a, b) && a->w == b->w; }
+// does a result share no memory with the tensors; null: not there
+bool apart(const mt_tensor *result, std::initializer_list<const mt_tensor *> tensors) {
+  for (auto t : tensors)
+    if (result && t && mt::overlap(result, t)) return false;
+  return true;
+}
 bool is_statistic(const mt_tensor *t, const mt_tensor *in, const Geometry &g) { return t->w == in->w && t->z == g.kept_z && t->y == g.kept_y && t->x == 1; }
 
 // rows of up to this many values are held in registers.  In the backward pass 1024 threads have room for 16 values each and their share
@@ -1110,9 +1117,9 @@ int backward_checks(const char *name, const mt_tensor *error, const mt_tensor *d
   for (auto t : {dgamma, dbeta})
     if (t && (mt::bad(t) || !same_sizes(t, gamma))) return mt::fail(MT_E_SHAPE, "%s: gradients must have the sizes of gamma", name);
   if (error->p != delta->p && mt::overlap(error, delta)) return mt::fail(MT_E_ARGUMENT, "%s: the error shares a part of its memory with delta", name);
-  for (auto out : {error, dgamma, dbeta})
-    for (auto t : {gamma, *func != MT_F_NONE ? beta : nullptr, mean, ivar, out == error ? nullptr : delta, out == error ? nullptr : error, out == dbeta ? dgamma : nullptr})
-      if (out && t && mt::overlap(out, t)) return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with another tensor", name);
+  const mt_tensor *read = *func != MT_F_NONE ? beta : nullptr;
+  if (!apart(error, {gamma, read, mean, ivar}) || !apart(dgamma, {gamma, read, mean, ivar, delta, error}) || !apart(dbeta, {gamma, read, mean, ivar, delta, error, dgamma}))
+    return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with another tensor", name);
   return MT_OK;
 }
 
@@ -1145,9 +1152,8 @@ int mt_layernorm_forward_func(const mt_tensor *out, const mt_tensor *in, const m
   for (auto t : {mean, ivar})
     if (t && !is_statistic(t, in, g)) return mt::fail(MT_E_SHAPE, "%s: mean and ivar must hold one value per row", name);
   if (out->p != in->p && mt::overlap(out, in)) return mt::fail(MT_E_ARGUMENT, "%s: the output shares a part of its memory with the input", name);
-  for (auto r : {out, mean, ivar})
-    for (auto t : {gamma, beta, r == out ? nullptr : in, r == out ? nullptr : out, r == ivar ? mean : nullptr})
-      if (r && t && mt::overlap(r, t)) return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with another tensor", name);
+  if (!apart(out, {gamma, beta}) || !apart(mean, {gamma, beta, in, out}) || !apart(ivar, {gamma, beta, in, out, mean}))
+    return mt::fail(MT_E_ARGUMENT, "%s: a result shares memory with another tensor", name);
   PackedView packed{};
   if (packed_input) {
     if (mt::bad(packed_input)) return mt::fail(MT_E_ARGUMENT, "%s: packed memory that is null or not 16-byte aligned", name);

@@ -1006,12 +1006,15 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
   a.error = error->p; a.dgamma = dgamma ? dgamma->p : nullptr; a.dbeta = dbeta ? dbeta->p : nullptr;
   a.delta = delta->p; a.gamma = gamma->p; a.beta = beta ? beta->p : nullptr; a.mean = mean->p; a.ivar = ivar->p;
   a.rows = g.rows; a.N = g.N; a.func = func; a.accumulate = accumulate != 0;
+  const Backward given = a;
   if (func == MT_F_GELU) {
-    ln_front_kernel<<<dim3(g.rows < 4096 ? g.rows : 4096, g.N < 65536 ? 1 : 16), THREADS, 0, mt::stream()>>>(a, x);
-    MT_LAUNCH_CHECK(name);
     a.delta = a.error;
     a.func = MT_F_NONE;
   }
+  // the first launch, once nothing can be refused any more: it writes over the error, which may be delta
+  const auto front = [&] {
+    if (func == MT_F_GELU) ln_front_kernel<<<dim3(g.rows < 4096 ? g.rows : 4096, g.N < 65536 ? 1 : 16), THREADS, 0, mt::stream()>>>(given, x);
+  };
   const bool params = dgamma || dbeta;
   const bool whole = g.N % 4 == 0 && x_aligned && aligned16(a.error) && aligned16(a.delta) && aligned16(a.gamma) && (a.func == MT_F_NONE || aligned16(a.beta));
   // (half of what the pass moves stands for the size of a tensor that is read and written: 4096 x 6144 62.6 -> 58.2 us)
@@ -1029,6 +1032,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
       if constexpr (L * E <= (int)BACKWARD_ROW) {
         const uint32_t per_block = L < 256 ? 256 / L : 1, threads = L < 256 ? 256 : L;
         if (beside) {
+          front();
           const uint32_t error_blocks = cdiv(g.rows, per_block), param_blocks = params ? cdiv(g.N, threads / 16) : 0;
           const auto go = [&](uint32_t first_row, uint32_t grid, uint32_t first_param_block) {
             with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
@@ -1055,6 +1059,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
         if (parts > 256) parts = 256;
         int rc = ln_workspace(2 * (size_t)parts * g.N, &partial);
         if (rc) return rc;
+        front();
         with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
           constexpr int ACCESS = decltype(v)::value;
           constexpr bool FUNC = decltype(f)::value;
@@ -1084,6 +1089,7 @@ int backward(const char *name, const mt_tensor *error, const mt_tensor *dgamma, 
     float2 *piece_sums = reinterpret_cast<float2 *>(ws);
     partial = ws + sums;
     parts = groups > 1 ? groups : 0;
+    front();
     with_kind(access, a.func != MT_F_NONE, [&](auto v, auto f) {
       constexpr int ACCESS = decltype(v)::value;
       constexpr bool FUNC = decltype(f)::value;

@@ -1,8 +1,8 @@
-"""Results of the layer norm that are one and the same tensor: refused like any other two that share memory.  Host-side checks, no device
-needed."""
+"""Results of the layer norm that are one and the same tensor, refused like any other two that share memory, and refusals in front of
+the first launch.  Host-side checks, no device needed."""
 import pytest
 
-from test_packed_refusals import ARGUMENT, fake, mt, refused  # noqa: F401 (fixtures)
+from test_packed_refusals import ARGUMENT, UNAVAILABLE, fake, mt, refused  # noqa: F401 (fixtures)
 
 
 def test_one_tensor_as_output_and_statistic(mt, fake):  # noqa: F811
@@ -31,3 +31,17 @@ def test_one_tensor_as_error_and_gradient(mt, fake, packed):  # noqa: F811
     refused(mt, ARGUMENT, "memory", f, delta, delta, dbeta, delta, gamma, x, mean, ivar)
     refused(mt, ARGUMENT, "memory", f, error, dgamma, dgamma, delta, gamma, x, mean, ivar)
     refused(mt, ARGUMENT, "memory", f, gamma, dgamma, dbeta, delta, gamma, x, mean, ivar)
+
+
+def test_nothing_is_launched_before_a_refusal(mt):  # noqa: F811
+    """More long rows than one launch takes: said before GeLU's derivative is written into the error."""
+    at = [1 << 44]
+
+    def tensor(*shape):
+        at[0] += 1 << 42
+        return mt.CTensor.wrap(at[0], shape)
+
+    rows, n = 3_400_000, 20000
+    for func in (None, "gelu"):
+        args = [tensor(rows, 1, n, 1), tensor(1, 1, n, 1), tensor(1, 1, n, 1), tensor(rows, 1, n, 1), tensor(1, 1, n, 1), tensor(rows, 1, n, 1), tensor(rows, 1, 1, 1), tensor(rows, 1, 1, 1)]
+        refused(mt, UNAVAILABLE, "too many", mt.Fused.LayerNormBackward, *args, beta=tensor(1, 1, n, 1), func=func)

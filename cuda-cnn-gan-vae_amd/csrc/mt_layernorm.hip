@@ -5,7 +5,7 @@
 //   error = ivar * (u - sum(u) / N - xhat * sum(u * xhat) / N),  dgamma = sum over the rows of g * xhat,  dbeta = of g
 //
 // All of it is bound by memory: the forward pass has to read x and write y, the backward pass to read delta and x and write the
-// error.  A row is therefore held in registers between its sums and its results wherever it fits (one to 1024 threads per row, up
+// error.  A row is therefore held in registers between its sums and its results wherever it fits (8 to 1024 threads per row, up
 // to 32 values per thread); longer rows are cut into pieces that several blocks share, and their second look at x finds it in
 // the caches.  Variances are sums of squared deviations from the mean (two passes over registers), never E[x^2] - E[x]^2.
 #include <initializer_list>

@@ -166,7 +166,9 @@ int mt_timer_destroy(void *timer);
  *                    block, 2 the same with two groups of wavefronts, 3 256 rows (an even number of features, else 2), all in three
  *                    bf16 numbers; 4 and 5 as 2 and 3 in two fp16 numbers -- and the batch in s parts (0: one; 128 at most)
  *   "nontemporal"    2 (default) the re-sampling, pooling, large-batch batch-norm, layer-norm and 8-bit packing kernels read and
- *                    write tensors of 128 MiB and more past the caches (each element is touched once) / 1 always / 0 never
+ *                    write tensors of 128 MiB and more past the caches (each element is touched once; the layer norm's backward pass,
+ *                    which moves two tensors and an input, where half of what it moves is that much: delta of 85 1/3 MiB and
+ *                    more with an fp32 input, of 113 7/9 MiB from 8 bits) / 1 always / 0 never
  *   "staged_uploads" 1 (default) mt_copy_h2d of at most 64 KiB copies the caller's buffer into a pinned slot at once and queues
  *                    the copy to the device behind the work already queued, without waiting for it / 0 every upload waits
  *   "pool"           1 (default) mt_free keeps blocks for the next mt_malloc of the same size (stream-ordered reuse, no
@@ -400,12 +402,16 @@ int mt_convolution_backward_weights_sum(const mt_tensor *dkernel, int32_t dkerne
  * gamma names the row: [1,Z,Y,X] of the input's sizes (a row is a whole sample), [1,1,Y,X] (a plane; the features of a
  * linear layer's output [B,1,Out,1]) or [1,1,1,X].  With N values per row:
  *   mean = sum(x)/N, ivar = 1/sqrt(sum((x-mean)^2)/N + epsilon), xhat = (x-mean)*ivar, output = func(gamma*xhat + beta).
- * mean and ivar hold one value per row: the input's sizes with 1 in place of those that the row spans.  Sums are fp32, taken in
- * an order that depends on the sizes and on whether the tensors are 16-byte aligned: the same call gives the same bits.
+ * mean and ivar hold one value per row: the input's sizes with 1 in place of those that the row spans.  Sums are fp32.  The same
+ * call gives the same bits; their order depends on N, on whether the tensors are 16-byte aligned and, for rows of 129 to 1023 values that are no
+ * multiple of four, on whether packed_input is given.  So a row's mean, ivar and output are the same in every batch.  In the backward
+ * pass the order of the sums over the rows depends on their number, and the last bits of a row's error do too, and depend on whether
+ * dgamma or dbeta is given, where rows have 8193 to 16384 values.
  * A NaN or an infinity in a row makes that row of xhat NaN, and with it the row's error and the dgamma it adds to (what func
- * makes of a NaN is its own: MT_F_RELU makes it 0).  Values whose squared deviations overflow (1.8e19 from their mean) have an
- * ivar of 0.  At most 2^31 - 1 rows, of at most 2^31 - 17 values; the backward pass takes fewer than 2^36 values in
- * all where the rows are longer than 8192.
+ * makes of a NaN is its own: MT_F_RELU makes it 0), and so do finite values whose sum over the row, or over a part of it, is more than
+ * fp32 holds, and an epsilon of 0 in a row of equal values.  Values whose squared deviations overflow (1.8e19 from their mean) have an
+ * ivar of 0.  At most 2^31 - 1 rows, of at most 2^31 - 17 values; the backward pass of rows longer than 8192 may refuse 2^24 and more pieces
+ * of 4096 values (what is left of a row counts as one).
  * No result may share memory with another tensor, but for the two cases named below.
  *
  * mt_layernorm_forward_func: mean and ivar (NULL to skip) are what the backward pass needs.  output may be the same tensor as
@@ -432,7 +438,8 @@ int mt_layernorm_backward_packed_func(const mt_tensor *error, const mt_tensor *d
  * No counterpart in the reference.  A training step keeps every layer's input until the backward pass; kept in 8 bits it takes
  * 1.0625 bytes per element instead of 4.  128 consecutive elements of a sample (its Z*Y*X values in memory order; the last
  * group of a sample may be shorter) share a lowest value and a step:
- *   low = min, step = (max - low) * (1/255), q = (x - low) / step rounded to a whole number (half to even), 0..255,
+ *   low = min, step = (max - low) * (1/255), q = (x - low) * (1/step) rounded to a whole number (half to even), 0..255, 1/step rounded
+ *   to fp32 first (beside half a step that can be the other of two neighbours),
  *   value = low + step*q, computed in fp32: |value - x| <= step/2 and the rounding of the sum.
  * A group of equal values comes back exactly; one whose range is below 3e-36 as its lowest value.  A group whose range is not a
  * finite number (it holds a NaN or an infinity, or values 3.4e38 apart) comes back as NaN in every element.

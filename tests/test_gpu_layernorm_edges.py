@@ -128,3 +128,49 @@ def test_gradients_against_differences(mt, n, func):
         moves = np.linalg.norm(weight * (ends[0] - ends[1]) / (2 * h))
         slack = 4 * 2e-6 * moves + 1e-6 * np.abs(got[key] * direction).sum() + 1e-9 * np.abs(weight).sum()
         assert abs(slope - mine) <= slack + kinks, key
+
+
+@pytest.mark.parametrize("n", [1024, 4096, 40000])
+def test_a_sum_that_overflows(mt, n):
+    """Finite values whose sum fp32 does not hold: NaN, in that row alone."""
+    shape, pshape = (3, 1, n, 1), (1, 1, n, 1)
+    x, gamma, beta, delta = inputs(n, shape, pshape)
+    clean = run_forward(mt, x, gamma, beta)
+    x[1] = 1e36
+    out, mean, ivar, _ = run_forward(mt, x, gamma, beta)
+    assert np.isnan(out[1]).all() and not np.isfinite(mean[1]).any() and np.array_equal(out[[0, 2]], clean[0][[0, 2]])
+    assert np.isnan(run_backward(mt, delta, x, gamma, beta, mean, ivar)["error"][1]).all()
+
+
+@pytest.mark.parametrize("n", [130, 333, 1001, 1023])
+def test_the_8_bit_copy_beside_rows_of_odd_length(mt, n):
+    """Such rows are summed in another order when the input is kept in 8 bits on the way: within the bounds both times."""
+    x, gamma, beta, _ = inputs(n, (40, 1, n, 1), (1, 1, n, 1))
+    want = po.forward(x, gamma, beta, 1e-6, "tangence")
+    for packed in (False, True):
+        for key, got in zip(("out", "mean", "ivar"), run_forward(mt, x, gamma, beta, "tangence", packed=packed)):
+            within(got, want, key)
+
+
+@pytest.mark.parametrize("n", [8193, 10319, 16384])
+@pytest.mark.parametrize("func", [None, "sigmoid"])
+def test_the_error_with_other_arguments(mt, n, func):
+    """Rows of 8193 to 16384 values take other kernels with the number of rows and with the gradients that are wanted: the error of a row
+    within its bounds whatever is asked for beside it."""
+    rows = 1100
+    x, gamma, beta, delta = inputs(n, (rows, 1, n, 1), (1, 1, n, 1))
+    _, mean, ivar, pk = run_forward(mt, x, gamma, beta, func, packed=True)
+    tg, tb = up(mt, gamma), up(mt, beta)
+    for kept in (False, True):
+        back = po.backward(delta, po.through_8_bits(x) if kept else x, gamma, beta, mean, ivar, func)
+        for count in (rows, 600, 7):
+            part = {key: back[key][:count] for key in ("error", "error_tol")}
+            source = up(mt, x[:count])
+            if kept:
+                source = mt.CPackedTensor(count, 1, n, 1)
+                mt.CTensorMath.Pack(source, up(mt, x[:count]))
+            for wanted in (True, False):
+                error = mt.CTensor(count, 1, n, 1)
+                grads = (mt.CTensor(*gamma.shape), mt.CTensor(*gamma.shape)) if wanted else (None, None)
+                mt.Fused.LayerNormBackward(error, *grads, up(mt, delta[:count]), tg, source, up(mt, mean[:count]), up(mt, ivar[:count]), beta=tb, func=func, accumulate=False)
+                within(error.numpy(), part, "error")

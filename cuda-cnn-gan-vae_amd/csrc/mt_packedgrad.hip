@@ -22,9 +22,9 @@
 //   again with three numbers where it is not so.  The powers need a look at all of delta before (a launch that reads it once and sums
 //   the columns for dbias on the way), so this is for products that are worth it.
 // Three (two) 16-bit matrix instructions multiply what one fp32 product would, at a third (half) of a rate where the library's bf16
-// product reaches 1295 TFLOP/s; the fp32 matrix instructions reach 157 at most.  4096^3: 315 to 337 us in two numbers, 366 to 398 in
-// three (a chip that draws less power is faster: the clock falls to 1.9 GHz in these loops, and the matrix instructions of one wavefront
-// and the vector instructions of the other add up to 92 % of the cycles).  The second sum is one fp32 multiply-add per element of
+// product reaches 1295 TFLOP/s; the fp32 matrix instructions reach 157 at most.  4096^3: 310 to 326 us in two numbers, 363 to 372 in three; a block
+// that starts again takes both (651 us where all do).  The clock falls with the load: 603000 cycles per launch are 300 us at 2.0 GHz in
+// launches apart, 356 in twenty without a pause; the matrix cores work in 43 % of the cycles, the vector units in 47 %.  The second sum is one fp32 multiply-add per element of
 // delta on the way.
 //
 // A column tile is one group, so that a sample has one (low, step) in it.  A block is four wavefronts, each with its own 32 or
@@ -523,10 +523,10 @@ mt::Workspace g_wgrad_ws;
 // two groups of wavefronts per block, parts of the batch.  The estimate of each variant's time in microseconds is its fixed part plus
 // the steps that the busiest compute unit takes, at the measured time of a step with one or two blocks on it, plus writing and
 // joining the parts' sums; two fp16 numbers instead of three bf16 ones take 0.82 of the steps' time and a look at delta before.  Measured
-// against one another, in three numbers: 4096^3 366 us with 256 rows, 412 with 128; 2048^3 58 with 128 rows and two groups, 66 with one,
-// 72 with 256 rows and four parts; 1000 x 1000 x 1777 27.5 with two groups, 31.9 with two parts; 512^3 11.2 in four parts, 19 in
-// one.  In two numbers against three (on a slower chip): 4096^3 337 and 383, 8192 x 4096 x 1024 186 and 214, 2048^3 54.8 and 58.6,
-// 256 x 4096 x 4096 33.6 and 33.4, 512^3 15.3 and 11.2.
+// against one another, in three numbers: 4096^3 372 us with 256 rows, 407 with 128; 2048^3 59 with 128 rows and two groups, 66 with one,
+// 108 with 256 rows; 1777 samples, 1000 -> 1000 28.4 in four parts, 31.0 with two groups in two, 55 in one part; 512^3 11.4 in four parts, 18.4
+// in one.  In two numbers against three: 4096^3 314 and 372, 1024 samples, 4096 -> 8192 171 and 196, 2048^3 55.9 and 58.6, 256 x 4096 x 4096
+// 34.0 and 33.6, 512^3 18.7 and 15.7.
 struct Plan {
   uint32_t rows, split;
   bool pair, half;

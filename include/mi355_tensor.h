@@ -452,7 +452,9 @@ int mt_unpack(const mt_tensor *output, const mt_packed_tensor *input);          
  * dweight [1,1,Out,In] (+)= sum over the batch of delta (x) value(input), dbias [1,1,Out,1] (NULL to skip) (+)= sum of delta;
  * input [B,...] of In values per sample, delta [B,...] of Out values.  accumulate: 1 adds to what the gradients hold, 0 overwrites.
  * delta*step is an fp32 number, or (large layers, where the time that it saves pays for a look at all of delta before) one whose
- * error is at most 2^-23 of itself, or 2^-26 of the largest delta*step that its row of dweight meets in its 128 columns;
+ * error is at most 2^-23 of itself, or 2^-26 of the largest delta*step that its row of dweight meets in its 128 columns (where that is far
+ * below the product of the row's largest delta and the columns' largest step, as padded samples may make it, the fp32 form is taken after
+ * all, and the call takes up to twice its time);
  * its products with whole numbers, q less the count that stands for 0 in its group, are exact and summed in fp32: values of 0 in a group whose
  * lowest value is 0 (what a ReLU leaves) add exactly nothing.  The same call gives the same bits.  A delta that is not a
  * finite number makes its row of dweight NaN; one whose product with a step is beyond fp32's range leaves a NaN, an infinity or what the

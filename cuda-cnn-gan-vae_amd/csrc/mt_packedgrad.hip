@@ -51,6 +51,7 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4_of_any __attribute__((ext_vector_type(4), may_alias));
 
 // the next rows of an operand, at most `most` of the `left` that there are (none: left <= 0): what lies behind them reads as
 // zero.  most * row_bytes <= 2^30: 16 rows of delta or dweight, 64 of the packed bytes, fewer than 2^24 features.
@@ -138,9 +139,10 @@ __device__ __forceinline__ void packed_wgrad_loop(const WgradArgs &a, uint32_t g
     const float low = __uint_as_float(pair.x), step = __uint_as_float(pair.y);
     const float zero = fminf(fmaxf(rintf(-low * (step > 0.f ? mt::reciprocal(step) : 0.f)), 0.f), 255.f);
     zeros[tid / 64u][lane] = (uint16_t)zero;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (no instruction: the compiler must not take the load for one of other memory)
     __builtin_amdgcn_wave_barrier();
-    const uintx4 z = *reinterpret_cast<const uintx4 *>(&zeros[tid / 64u][kg * 8u]);
-    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const uintx4 z = *reinterpret_cast<const uintx4_of_any *>(&zeros[tid / 64u][kg * 8u]);
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       uintx4 w;
